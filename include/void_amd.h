@@ -388,6 +388,28 @@ int void_sddmm_rows_f16(const void* grad_c, int64_t ldg, const void* b, int64_t 
                         int32_t n_groups, const int32_t* col_idx, const int64_t* tile_index, int32_t M, int32_t N,
                         int32_t K, void* grad_tiles, int32_t out_dtype, hipStream_t stream);
 
+/* ---- Layer norm -------------------------------------------------------- */
+
+/* y = (x - mu) / sqrt(v + eps) * weight + bias over rows of `cols` values, mu
+ * and v the row's mean and (biased) variance in fp32.  x and y have `dtype`
+ * (f32, bf16, f16), rows ldx and ldy elements apart; weight and bias (each may
+ * be null: 1 and 0) have `param_dtype`, which is dtype or f32.  stats (or null)
+ * receives (mu, 1 / sqrt(v + eps)) per row, 8-byte aligned, for the gradient.
+ * Any width and any alignment of whole elements; x may have ldx 0 (one row
+ * repeated).  x and y may be the same array.  No counterpart in the reference. */
+int void_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, int32_t param_dtype, int64_t rows,
+                    int32_t cols, float eps, int32_t dtype, void* y, int64_t ldy, float* stats, hipStream_t stream);
+
+/* Its gradient: dx [rows, cols] of dtype, dweight and dbias [cols] of
+ * param_dtype; each may be null and is then not computed.  The workspace
+ * (void_layer_norm_grad_workspace_bytes, no initial contents) is needed where
+ * dweight or dbias is; sums run in a fixed order. */
+size_t void_layer_norm_grad_workspace_bytes(int64_t rows, int32_t cols, int32_t dtype);
+int void_layer_norm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
+                         int32_t param_dtype, const float* stats, int64_t rows, int32_t cols, int32_t dtype, void* dx,
+                         int64_t lddx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                         hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -144,6 +144,12 @@ SIGNATURES = {
                                       c_void_p]),
     "void_csr_to_tiles": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_size_t,
                                   ctypes.c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "void_layer_norm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_float, c_int32,
+                                c_void_p, c_int64, c_void_p, c_void_p]),
+    "void_layer_norm_grad_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32]),
+    "void_layer_norm_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_int64,
+                                     c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t,
+                                     c_void_p]),
 }
 
 _lock = threading.Lock()

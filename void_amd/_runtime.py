@@ -57,6 +57,24 @@ def vector_f32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t.reshape(-1).to(device=device, dtype=torch.float32).contiguous()
 
 
+FLOAT_CODES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def float_code(t: torch.Tensor, what: str) -> int:
+    """The library's code of t's dtype; TypeError unless it is fp32, bf16 or fp16."""
+    code = FLOAT_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def flat_rows(t: torch.Tensor) -> torch.Tensor:
+    """t as a 2-D tensor of its last axis's rows with unit column stride; a
+    view wherever the strides allow one (rows of any pitch, one row repeated)."""
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
 class StreamWorkspaces:
     """One split-row workspace for each HIP stream, for all plans of the
     differentiable SpMM: their launches on one stream run in order, so they can

@@ -11,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -20,7 +22,8 @@ INCLUDE_DIR = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libvoid_amd.so"
 ARCH = "gfx950"
 
-SOURCES = [SRC_DIR / "void_spmm.hip", SRC_DIR / "void_quant.hip", SRC_DIR / "void_format.hip", SRC_DIR / "void_sddmm.hip"]
+SOURCES = [SRC_DIR / "void_spmm.hip", SRC_DIR / "void_quant.hip", SRC_DIR / "void_format.hip", SRC_DIR / "void_sddmm.hip",
+           SRC_DIR / "void_norm.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -67,13 +70,24 @@ def build(verbose: bool = False, clock_probe: bool = False, phase_probe: bool = 
     out = CLOCK_LIB_PATH if clock_probe else PHASE_LIB_PATH if phase_probe else LIB_PATH
     tmp = out.with_suffix(".so.tmp")
     extra = CLOCK_FLAGS if clock_probe else PHASE_FLAGS if phase_probe else []
-    cmd = [hipcc(), *HIPCC_FLAGS, *extra, f"-I{INCLUDE_DIR}", *map(str, SOURCES), "-o", str(tmp)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError(f"hipcc failed with exit code {proc.returncode}")
+
+    def run(args):
+        cmd = [hipcc(), *args]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            sys.stderr.write(proc.stdout + proc.stderr)
+            raise RuntimeError(f"hipcc failed with exit code {proc.returncode}")
+
+    # One compiler a source, together: the build takes as long as its longest source.
+    with tempfile.TemporaryDirectory() as d:
+        objects = [str(Path(d) / (src.stem + ".o")) for src in SOURCES]
+        compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            list(pool.map(lambda so: run([*compile_flags, *extra, f"-I{INCLUDE_DIR}", "-c", str(so[0]), "-o", so[1]]),
+                          zip(SOURCES, objects)))
+        run([f"--offload-arch={ARCH}", "-shared", "-fPIC", *objects, "-o", str(tmp)])
     os.replace(tmp, out)
     return out
 

@@ -1,0 +1,120 @@
+// rows.h — 16-byte pieces of float rows and sums over the threads of a row,
+// shared by the layer norm, distillation and dense layer kernels.
+//
+// A piece is 16 bytes of a row: 8 bf16 / fp16 values or 4 fp32 values.  Rows
+// need no alignment past their elements': global memory takes 16-byte accesses
+// at any element address, so a row of any width and pitch is read and written
+// in whole pieces, and only the piece that the row ends in goes by elements.
+
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace {
+
+template <class E>
+struct Piece {
+  static constexpr int n = 16 / (int)sizeof(E);
+  typedef E vec __attribute__((ext_vector_type(16 / sizeof(E))));
+  typedef float fvec __attribute__((ext_vector_type(16 / sizeof(E))));
+  typedef vec any __attribute__((aligned(sizeof(E))));
+};
+
+// The piece of a row of `cols` values that starts at column c; zeros past the end.
+template <class E>
+__device__ __forceinline__ typename Piece<E>::vec load_piece(const E* row, int c, int cols) {
+  typename Piece<E>::vec v = {};
+  if (c + Piece<E>::n <= cols) {
+    v = *reinterpret_cast<const typename Piece<E>::any*>(row + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < Piece<E>::n; ++e)
+      if (c + e < cols) v[e] = row[c + e];
+  }
+  return v;
+}
+
+template <class E>
+__device__ __forceinline__ void store_piece(E* row, int c, int cols, typename Piece<E>::vec v) {
+  if (c + Piece<E>::n <= cols) {
+    *reinterpret_cast<typename Piece<E>::any*>(row + c) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < Piece<E>::n; ++e)
+      if (c + e < cols) row[c + e] = v[e];
+  }
+}
+
+// n values of a parameter vector (weight, bias) from column c, in fp32; `none`
+// stands for each where there is no vector, zero past the end.
+template <int N, class W>
+__device__ __forceinline__ void load_params(float (&f)[N], const W* p, int c, int cols, float none) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = none;
+  } else if (c + N <= cols) {
+#pragma unroll
+    for (int q = 0; q < N; q += Piece<W>::n <= N ? Piece<W>::n : N) {
+      constexpr int n = Piece<W>::n <= N ? Piece<W>::n : N;
+      typedef W vec __attribute__((ext_vector_type(n)));
+      typedef vec any __attribute__((aligned(sizeof(W))));
+      const vec v = *reinterpret_cast<const any*>(p + c + q);
+#pragma unroll
+      for (int e = 0; e < n; ++e) f[q + e] = (float)v[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = c + e < cols ? (float)p[c + e] : 0.f;
+  }
+}
+
+// Sum over the aligned group of T lanes (a power of two up to 64) that holds this lane.
+template <int T>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int off = T / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// Sums of a (and b) over the T threads of a row: T up to 64 lanes, or the whole
+// workgroup of T threads through LDS.  Two areas of `red` in turn, so that one
+// barrier a sum is enough: area i is written again only behind the barrier of
+// the sum in between, which every thread reaches after its reads of area i.
+template <int T>
+struct RowSum {
+  float2 (*red)[16];
+  int turn = 0;
+  __device__ __forceinline__ float2 sum(float a, float b) {
+    a = lanes_sum<(T < 64 ? T : 64)>(a);
+    b = lanes_sum<(T < 64 ? T : 64)>(b);
+    if constexpr (T > 64) {
+      if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = make_float2(a, b);
+      __syncthreads();
+      a = b = 0.f;
+#pragma unroll
+      for (int w = 0; w < T / 64; ++w) {
+        const float2 r = red[turn][w];
+        a += r.x;
+        b += r.y;
+      }
+      turn ^= 1;
+    }
+    return make_float2(a, b);
+  }
+  __device__ __forceinline__ float sum(float a) {
+    a = lanes_sum<(T < 64 ? T : 64)>(a);
+    if constexpr (T > 64) {
+      if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6].x = a;
+      __syncthreads();
+      a = 0.f;
+#pragma unroll
+      for (int w = 0; w < T / 64; ++w) a += red[turn][w].x;
+      turn ^= 1;
+    }
+    return a;
+  }
+};
+
+}  // namespace
