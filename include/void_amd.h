@@ -410,6 +410,55 @@ int void_layer_norm_grad(const void* dy, int64_t lddy, const void* x, int64_t ld
                          int64_t lddx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
                          hipStream_t stream);
 
+/* ---- Distillation from a teacher's top logits -------------------------- */
+
+#define VOID_DISTILL_MAX_ENTRIES 1024
+
+/* rows x vocab student logits, and per row k teacher entries (logit, index).
+ * Entries with a negative index or a logit of -inf do not count; an index of
+ * vocab or more makes its row's loss and gradient NaN. */
+typedef struct void_distill_args {
+  const void* logits;    /* rows ld elements apart, of dtype (f32, bf16, f16) */
+  int64_t ld;
+  const void* teacher;   /* [rows, k] logits, rows ldt elements apart, of teacher_dtype */
+  int64_t ldt;
+  const void* index;     /* [rows, k] int32 or int64 (index_bytes), rows ldi elements apart */
+  int64_t ldi;
+  int64_t rows;
+  int32_t vocab, k;      /* k <= VOID_DISTILL_MAX_ENTRIES */
+  int32_t dtype, teacher_dtype, index_bytes;
+  float temperature;
+} void_distill_args;
+
+/* Slices that a row's sums are made in (few rows, long vocabulary); at most 64. */
+int32_t void_distill_slices(int64_t rows, int32_t vocab);
+
+/* With p = softmax(teacher / T) over a row's entries and q = softmax(logits / T)
+ * over the vocabulary: row_loss[r] = T^2 sum_j p_j (log p_j - log q_{index_j}),
+ * 0 for a row without entries; used[r] = whether it has any.  parts
+ * ([rows][void_distill_slices()][2], 8-byte aligned) receives each slice's
+ * largest logit m and sum of exp((logit - m) / T), for the gradient.  No
+ * counterpart in the reference. */
+int void_distill_loss(const void_distill_args* d, float* row_loss, float* parts, int32_t* used, hipStream_t stream);
+
+/* *loss = sum of the rows' losses times *factor (which may be null and is not
+ * read), factor = 1, or for the mean 1 / the number of used rows (at least 1). */
+int void_distill_reduce(const float* row_loss, const int32_t* used, int64_t rows, int32_t mean, float* loss,
+                        float* factor, hipStream_t stream);
+
+/* grad[r][v] = upstream[r upstream_step] * *factor (1 where null) * T (q_v -
+ * sum of p_j with index_j = v), of d->dtype, rows ldg elements apart; zero for
+ * rows without entries.  parts from void_distill_loss.  grad must not overlap
+ * the logits. */
+int void_distill_grad(const void_distill_args* d, const float* parts, const float* upstream, int64_t upstream_step,
+                      const float* factor, void* grad, int64_t ldg, hipStream_t stream);
+
+/* Loss (sum, or mean over the used rows) and grad_scale times its gradient in
+ * one go: the logits are read once.  The workspace has no initial contents. */
+size_t void_distill_step_workspace_bytes(int64_t rows, int32_t vocab);
+int void_distill_step(const void_distill_args* d, int32_t mean, float grad_scale, float* loss, void* grad, int64_t ldg,
+                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

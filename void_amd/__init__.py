@@ -49,6 +49,7 @@ from .fusion import (ActivationType, FusedSparseLinear, get_activation_code, voi
 from .packed import load_packed, pack, save_packed, unpack
 from .ops import MIN_TENSOR_CORE_K, compute_optimal_tile_n, void_spmm
 from .autograd import SparseLinear, VOIDSpMM, VOIDSpMMFunction
+from .distill import distillation_loss, distillation_loss_and_grad
 from .norm import LayerNorm, layer_norm
 from .stream_k import StreamKWorkload, analyze_workload_balance, compute_stream_k_workload, void_spmm_stream_k
 
@@ -65,5 +66,6 @@ __all__ = [
     "ActivationType", "get_activation_code", "void_spmm_gelu", "void_spmm_relu", "void_spmm_silu",
     "StreamKWorkload", "compute_stream_k_workload", "analyze_workload_balance", "void_spmm_stream_k",
     "void_spmm", "compute_optimal_tile_n", "MIN_TENSOR_CORE_K", "FusedSparseLinear", "SparseLinear", "VOIDSpMM",
-    "VOIDSpMMFunction", "layer_norm", "LayerNorm", "pack", "unpack", "save_packed", "load_packed",
+    "VOIDSpMMFunction", "layer_norm", "LayerNorm", "distillation_loss",
+    "distillation_loss_and_grad", "pack", "unpack", "save_packed", "load_packed",
 ]

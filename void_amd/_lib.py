@@ -97,6 +97,24 @@ class DenseArgs(ctypes.Structure):
     ]
 
 
+class DistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p),
+        ("ld", c_int64),
+        ("teacher", c_void_p),
+        ("ldt", c_int64),
+        ("index", c_void_p),
+        ("ldi", c_int64),
+        ("rows", c_int64),
+        ("vocab", c_int32),
+        ("k", c_int32),
+        ("dtype", c_int32),
+        ("teacher_dtype", c_int32),
+        ("index_bytes", c_int32),
+        ("temperature", c_float),
+    ]
+
+
 # Every symbol include/void_amd.h declares, with its ctypes signature.
 SIGNATURES = {
     "void_abi_version": (c_int, []),
@@ -150,6 +168,14 @@ SIGNATURES = {
     "void_layer_norm_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_int64,
                                      c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t,
                                      c_void_p]),
+    "void_distill_slices": (c_int32, [c_int64, c_int32]),
+    "void_distill_loss": (c_int, [POINTER(DistillArgs), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "void_distill_reduce": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p]),
+    "void_distill_grad": (c_int, [POINTER(DistillArgs), c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                  c_void_p]),
+    "void_distill_step_workspace_bytes": (c_size_t, [c_int64, c_int32]),
+    "void_distill_step": (c_int, [POINTER(DistillArgs), c_int32, c_float, c_void_p, c_void_p, c_int64, c_void_p,
+                                  c_size_t, c_void_p]),
 }
 
 _lock = threading.Lock()
