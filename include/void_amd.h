@@ -459,6 +459,61 @@ size_t void_distill_step_workspace_bytes(int64_t rows, int32_t vocab);
 int void_distill_step(const void_distill_args* d, int32_t mean, float grad_scale, float* loss, void* grad, int64_t ldg,
                       void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- Dense layer --------------------------------------------------------- */
+
+/* Z = X W^T + bias, Y = activation(Z) + residual.  X [M, K], W [N, K], residual
+ * and Y [M, N] have dtype (f32, bf16, f16) with rows ld* elements apart; bias
+ * [N] has bias_dtype (dtype or f32).  bias, residual and slope may be null. */
+typedef struct void_linear_args {
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* y;
+  int64_t ldy;
+  void* slope;            /* [M, N] contiguous activation'(Z) for the gradient: fp32 for fp32
+                             values, else 2-byte codes; needs an activation */
+  void* workspace;
+  size_t workspace_bytes; /* void_linear_workspace_bytes(); no initial contents */
+  int64_t M, N, K;
+  int32_t dtype, bias_dtype;
+  int32_t activation;     /* void_activation */
+  int32_t reserved;
+} void_linear_args;
+
+/* Products of exact fp32 terms summed in fp32, one rounding of Y.  Up to 64 rows
+ * of X (void_linear_any_alignment() is 1) take operands of any alignment; more
+ * need X and W 16-byte aligned with K, ldx and ldw whole 16-byte chunks (else
+ * VOID_ERR_UNSUPPORTED).  Y may be the residual's array.  No counterpart in the
+ * reference. */
+int32_t void_linear_any_alignment(int64_t M);
+size_t void_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype);
+int void_linear(const void_linear_args* d, hipStream_t stream);
+
+/* dZ = dY activation'(Z) from the forward pass's slope, rows of whole 16-byte
+ * chunks whose tail past N is written as zero (dz null: not computed), and db =
+ * sum over rows of dZ (of dY where slope is null), of bias_dtype (db null: not
+ * computed).  The workspace is needed for db. */
+size_t void_linear_grad_z_workspace_bytes(int64_t M, int64_t N, int32_t dtype);
+int void_linear_grad_z(const void* dy, int64_t lddy, const void* slope, int64_t M, int64_t N, int32_t dtype, void* dz,
+                       int64_t ldz, void* db, int32_t bias_dtype, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+
+/* dX [M, K] = dZ [M, N] W [N, K] and dW [N, K] = dZ^T X.  dZ, W and X: 16-byte
+ * aligned rows of whole 16-byte chunks, dZ zero from N to the next chunk.  The
+ * workspace has void_linear_grad_workspace_bytes(rows and columns of the
+ * result, depth of the sum, dtype) bytes. */
+size_t void_linear_grad_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t dtype);
+int void_linear_grad_x(const void* dz, int64_t ldz, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K,
+                       int32_t dtype, void* dx, int64_t ldx, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+int void_linear_grad_w(const void* dz, int64_t ldz, const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K,
+                       int32_t dtype, void* dw, int64_t ldw, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

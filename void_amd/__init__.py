@@ -50,6 +50,7 @@ from .packed import load_packed, pack, save_packed, unpack
 from .ops import MIN_TENSOR_CORE_K, compute_optimal_tile_n, void_spmm
 from .autograd import SparseLinear, VOIDSpMM, VOIDSpMMFunction
 from .distill import distillation_loss, distillation_loss_and_grad
+from .linear import FusedLinear, fused_linear
 from .norm import LayerNorm, layer_norm
 from .stream_k import StreamKWorkload, analyze_workload_balance, compute_stream_k_workload, void_spmm_stream_k
 
@@ -67,5 +68,5 @@ __all__ = [
     "StreamKWorkload", "compute_stream_k_workload", "analyze_workload_balance", "void_spmm_stream_k",
     "void_spmm", "compute_optimal_tile_n", "MIN_TENSOR_CORE_K", "FusedSparseLinear", "SparseLinear", "VOIDSpMM",
     "VOIDSpMMFunction", "layer_norm", "LayerNorm", "distillation_loss",
-    "distillation_loss_and_grad", "pack", "unpack", "save_packed", "load_packed",
+    "distillation_loss_and_grad", "fused_linear", "FusedLinear", "pack", "unpack", "save_packed", "load_packed",
 ]

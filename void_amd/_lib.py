@@ -115,6 +115,30 @@ class DistillArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("ldx", c_int64),
+        ("w", c_void_p),
+        ("ldw", c_int64),
+        ("bias", c_void_p),
+        ("residual", c_void_p),
+        ("ldr", c_int64),
+        ("y", c_void_p),
+        ("ldy", c_int64),
+        ("slope", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+        ("M", c_int64),
+        ("N", c_int64),
+        ("K", c_int64),
+        ("dtype", c_int32),
+        ("bias_dtype", c_int32),
+        ("activation", c_int32),
+        ("reserved", c_int32),
+    ]
+
+
 # Every symbol include/void_amd.h declares, with its ctypes signature.
 SIGNATURES = {
     "void_abi_version": (c_int, []),
@@ -174,6 +198,17 @@ SIGNATURES = {
     "void_distill_grad": (c_int, [POINTER(DistillArgs), c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                                   c_void_p]),
     "void_distill_step_workspace_bytes": (c_size_t, [c_int64, c_int32]),
+    "void_linear_any_alignment": (c_int32, [c_int64]),
+    "void_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int32]),
+    "void_linear": (c_int, [POINTER(LinearArgs), c_void_p]),
+    "void_linear_grad_z_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32]),
+    "void_linear_grad_z": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                   c_int32, c_void_p, c_size_t, c_void_p]),
+    "void_linear_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int32]),
+    "void_linear_grad_x": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p,
+                                   c_int64, c_void_p, c_size_t, c_void_p]),
+    "void_linear_grad_w": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p,
+                                   c_int64, c_void_p, c_size_t, c_void_p]),
     "void_distill_step": (c_int, [POINTER(DistillArgs), c_int32, c_float, c_void_p, c_void_p, c_int64, c_void_p,
                                   c_size_t, c_void_p]),
 }

@@ -23,7 +23,7 @@ LIB_PATH = PKG_DIR / "libvoid_amd.so"
 ARCH = "gfx950"
 
 SOURCES = [SRC_DIR / "void_spmm.hip", SRC_DIR / "void_quant.hip", SRC_DIR / "void_format.hip", SRC_DIR / "void_sddmm.hip",
-           SRC_DIR / "void_norm.hip", SRC_DIR / "void_distill.hip"]
+           SRC_DIR / "void_norm.hip", SRC_DIR / "void_distill.hip", SRC_DIR / "void_linear.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

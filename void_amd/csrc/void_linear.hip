@@ -1,0 +1,756 @@
+// void_linear.hip — the dense layer with its epilogue, forward and backward,
+// for gfx950, declared in include/void_amd.h:
+//
+//   Z = X W^T + b,  Y = act(Z) + R;   dZ = dY act'(Z),  dX = dZ W,  dW = dZ^T X,
+//   db = sum_rows dZ.
+//
+// All three products are C[i][j] = sum_r A(i, r) B(j, r) with each operand
+// stored along r ("plain": X, W in the forward pass, dZ in dX) or along i / j
+// ("turned": W in dX; dZ and X in dW); one kernel takes every mix.  Products
+// run on the matrix cores (v_mfma_f32_32x32x16 for bf16 / fp16, 32x32x2 for
+// fp32: exact products, fp32 sums).
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <type_traits>
+
+#include "lds_dma.h"
+#include "rows.h"
+#include "void_amd.h"
+
+extern "C" __attribute__((visibility("hidden"))) int void_internal_fail(int code, const char* msg);
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef short v4h __attribute__((ext_vector_type(4)));
+typedef short v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
+
+// ---- epilogue --------------------------------------------------------------
+
+// act'(Z), kept for the backward pass: fp32 for fp32 values, else 16-bit fixed
+// point 2^15 s + 2^13 (s lies in [-0.13, 1.13] for every activation; 0 and 1 are
+// exact, others within 2^-16: a tenth of a bf16 rounding of dZ, where a slope
+// rounded to bf16 would add another whole one).  65535 stands for NaN.
+template <class E>
+struct Slope {
+  typedef uint16_t type;
+  static __device__ __forceinline__ uint16_t pack(float s) {
+    return s == s ? (uint16_t)(int)rintf(fmaf(s, 32768.f, 8192.f)) : (uint16_t)65535;
+  }
+  static __device__ __forceinline__ float unpack(uint16_t u) {
+    return u == 65535 ? __builtin_nanf("") : ((float)u - 8192.f) * (1.f / 32768.f);
+  }
+};
+template <>
+struct Slope<float> {
+  typedef float type;
+  static __device__ __forceinline__ float pack(float s) { return s; }
+  static __device__ __forceinline__ float unpack(float s) { return s; }
+};
+
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.442695040888963f));
+}
+
+// GELU in its tanh form: z sigmoid(2 u), u = 0.7978845608 (z + 0.044715 z^3).
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == VOID_ACT_RELU) return z < 0.f ? 0.f : z;
+  if (act == VOID_ACT_GELU) return z * sigmoid(1.5957691216f * z * fmaf(0.044715f * z, z, 1.f));
+  if (act == VOID_ACT_SILU) return z * sigmoid(z);
+  return z;
+}
+
+// Its derivative; beyond |z| = 30 it is 0 or 1 in fp32, and z^3 stays finite.
+__device__ __forceinline__ float slope_of(float z, int act) {
+  if (act == VOID_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  const float c = z > 30.f ? 30.f : z < -30.f ? -30.f : z;
+  if (act == VOID_ACT_GELU) {
+    const float s = sigmoid(1.5957691216f * c * fmaf(0.044715f * c, c, 1.f));
+    return fmaf(c * s * (1.f - s), 1.5957691216f * fmaf(0.134145f * c, c, 1.f), s);
+  }
+  const float s = sigmoid(c);
+  return fmaf(c * s, 1.f - s, s);
+}
+
+struct Epilogue {
+  void* out;             // [M, N] of E
+  int64_t ldo;
+  const void* bias;      // [N], or null
+  const void* residual;  // [M, N] of E, or null
+  int64_t ldr;
+  void* slope;           // [M, N] of Slope<E>, or null
+  int bias_f32, act;
+};
+
+template <class E>
+__device__ __forceinline__ float bias_at(const Epilogue& p, int64_t n) {
+  if (!p.bias) return 0.f;
+  return p.bias_f32 ? static_cast<const float*>(p.bias)[n] : (float)static_cast<const E*>(p.bias)[n];
+}
+
+template <class E>
+__device__ __forceinline__ void finish(const Epilogue& p, float sum, float bias, int64_t m, int64_t n, int64_t N) {
+  const float z = sum + bias;
+  if (p.slope) static_cast<typename Slope<E>::type*>(p.slope)[m * N + n] = Slope<E>::pack(slope_of(z, p.act));
+  float y = activate(z, p.act);
+  if (p.residual) y += (float)static_cast<const E*>(p.residual)[m * p.ldr + n];
+  static_cast<E*>(p.out)[m * p.ldo + n] = (E)y;
+}
+
+// The same for a piece of n values of a row from column c on.
+template <class E>
+__device__ __forceinline__ void finish_piece(const Epilogue& p, typename Piece<E>::fvec z, const float (&bias)[Piece<E>::n],
+                                             int64_t m, int c, int N) {
+  constexpr int n = Piece<E>::n;
+  typedef typename Piece<E>::fvec F;
+  typedef typename Slope<E>::type S;
+  typedef S SV __attribute__((ext_vector_type(16 / sizeof(E))));
+  typedef SV SAny __attribute__((aligned(sizeof(S))));
+#pragma unroll
+  for (int e = 0; e < n; ++e) z[e] += bias[e];
+  if (p.slope) {
+    S* sr = static_cast<S*>(p.slope) + m * N + c;
+    SV v;
+#pragma unroll
+    for (int e = 0; e < n; ++e) v[e] = Slope<E>::pack(slope_of(z[e], p.act));
+    if (c + n <= N) {
+      *reinterpret_cast<SAny*>(sr) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < n; ++e)
+        if (c + e < N) sr[e] = v[e];
+    }
+  }
+  if (p.act != VOID_ACT_NONE)
+#pragma unroll
+    for (int e = 0; e < n; ++e) z[e] = activate(z[e], p.act);
+  if (p.residual)
+    z += __builtin_convertvector(load_piece(static_cast<const E*>(p.residual) + m * p.ldr, c, N), F);
+  store_piece(static_cast<E*>(p.out) + m * p.ldo, c, N, __builtin_convertvector(z, typename Piece<E>::vec));
+}
+
+template <class E>
+__device__ __forceinline__ void bias_piece(const Epilogue& p, int c, int N, float (&f)[Piece<E>::n]) {
+  if (p.bias_f32) load_params(f, static_cast<const float*>(p.bias), c, N, 0.f);
+  else load_params(f, static_cast<const E*>(p.bias), c, N, 0.f);
+}
+
+// ---- the tiled product -----------------------------------------------------
+
+struct Product {
+  const void* a;  // plain: [M, K] rows lda apart; turned: [K, M]
+  const void* b;  // plain: [N, K]; turned: [K, N]
+  int64_t lda, ldb;
+  int64_t M, N, K;
+  int tiles_m, tiles_n, splits, steps_per_split;
+  float* part;  // splits > 1: [splits][M][N] fp32 sums instead of the epilogue
+  Epilogue epi;
+};
+
+__device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, float) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(v4f, a)[s], __builtin_bit_cast(v4f, b)[s], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0, 0, 0);
+}
+
+// One operand's B rows (of the tile) x 128 bytes along r, in LDS.
+//
+// Plain: row i at 128 i, its 16-byte chunks permuted by c ^ (i & 7), so that the
+// rows of a fragment read hit different banks.  Turned: row r of B values, its
+// chunks permuted by c ^ ((r & 3) << 2), for the transposing reads' 4 rows.  The
+// LDS-DMA writes lane after lane, so the permutation is in what each lane loads.
+template <class E, int B, int NW, bool TURNED>
+struct Operand {
+  static constexpr int kPer = 16 / (int)sizeof(E), kBK = 128 / (int)sizeof(E), kLoads = B * 128 / (NW * 1024);
+  static constexpr int kCpr = B * (int)sizeof(E) / 16;  // chunks of a turned row
+
+  const uint8_t* base;  // of the next step's first row / column
+  int64_t step;         // bytes from step to step
+  int voff[kLoads];
+  int at[kLoads];       // r of the load's chunk within a step
+
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int64_t i0, int64_t I, int64_t r0, int wave,
+                                       int lane) {
+    if constexpr (!TURNED) {
+      base = static_cast<const uint8_t*>(p) + (i0 * ld + r0) * (int64_t)sizeof(E);
+      step = 128;
+    } else {
+      base = static_cast<const uint8_t*>(p) + (r0 * ld + i0) * (int64_t)sizeof(E);
+      step = ld * 128;
+    }
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      const int id = (q * NW + wave) * 64 + lane;
+      if constexpr (!TURNED) {
+        const int row = id >> 3, c = (id & 7) ^ (row & 7);
+        voff[q] = i0 + row < I ? (int)(row * ld * (int64_t)sizeof(E)) + 16 * c : kOutOfRange;
+        at[q] = c * kPer;
+      } else {
+        const int row = id / kCpr, c = (id % kCpr) ^ ((row & 3) << 2);
+        voff[q] = i0 + c * kPer < I ? (int)(row * ld * (int64_t)sizeof(E)) + 16 * c : kOutOfRange;
+        at[q] = row;
+      }
+    }
+  }
+
+  // The next step into LDS; `left` values of r remain from it on.
+  __device__ __forceinline__ void load(uint8_t* lds, int wave, int left) {
+    const v4s r = sgpr_rsrc(base);
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) dma_b128(r, lds + (q * NW + wave) * 1024, at[q] < left ? voff[q] : kOutOfRange, 0);
+    base += step;
+  }
+
+  // Chunk pair kk's fragment of rows i0 .. i0 + 31: 16 bytes along r a lane.
+  static __device__ __forceinline__ v4i fragment(const uint8_t* lds, int i0, int kk, int lane) {
+    const int j = lane & 31, g = lane >> 5;
+    if constexpr (!TURNED) {
+      return *reinterpret_cast<const v4i*>(lds + (i0 + j) * 128 + (((2 * kk + g) ^ (j & 7)) << 4));
+    } else if constexpr (sizeof(E) == 4) {
+      v4f f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        f[s] = *reinterpret_cast<const float*>(lds + (8 * kk + 4 * g + s) * (B * 4) +
+                                               ((((i0 + j) >> 2) ^ (s << 2)) << 4) + (j & 3) * 4);
+      return __builtin_bit_cast(v4i, f);
+    } else {
+      // Two ds_read_b64_tr_b16: the 16 lanes of a read fetch 4 rows x 16 columns,
+      // 8 bytes each in row-major order, and lane t gets column t.
+      const int i = j & 15;
+      v4h t[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = 16 * kk + 8 * g + 4 * r + (i >> 2);
+        const int c = (i0 >> 3) + 2 * (j >> 4) + ((i & 3) >> 1);
+        const uint8_t* p = lds + row * (B * 2) + ((c ^ ((i >> 2) << 2)) << 4) + 8 * (i & 1);
+        t[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4h*)(const_cast<uint8_t*>(p)));
+      }
+      return __builtin_bit_cast(v4i, v8h{t[0][0], t[0][1], t[0][2], t[0][3], t[1][0], t[1][1], t[1][2], t[1][3]});
+    }
+  }
+};
+
+template <class E, int BM, int BN, int WR, int WC, bool TA, bool TB>
+__global__ __launch_bounds__(64 * WR * WC) void product_kernel(Product p) {
+  constexpr int NW = WR * WC, kBK = 128 / (int)sizeof(E), RA = BM / WR / 32, RB = BN / WC / 32;
+  typedef Operand<E, BM, NW, TA> OpA;
+  typedef Operand<E, BN, NW, TB> OpB;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][(BM + BN) * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups are dealt to the 8 XCDs in turn: each XCD gets a run of
+  // neighbouring tiles, whose operands its L2 then holds.
+  const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3;
+  int t = x * q + min(x, n & 7) + (blockIdx.x >> 3);
+  const int tiles = p.tiles_m * p.tiles_n, split = t / tiles;
+  t -= split * tiles;
+  constexpr int kGroup = 4;
+  const int group = t / (kGroup * p.tiles_n), first = group * kGroup, size = min(kGroup, p.tiles_m - first);
+  const int in = t - group * kGroup * p.tiles_n;
+  const int64_t m0 = (int64_t)(first + in % size) * BM, n0 = (int64_t)(in / size) * BN;
+
+  const int64_t r0 = (int64_t)split * p.steps_per_split * kBK;
+  const int64_t left = std::min<int64_t>(p.K - r0, (int64_t)p.steps_per_split * kBK);
+  const int steps = (int)((left + kBK - 1) / kBK);
+  OpA a;
+  OpB b;
+  a.init(p.a, p.lda, m0, p.M, r0, wave, lane);
+  b.init(p.b, p.ldb, n0, p.N, r0, wave, lane);
+  const int wm = (wave / WC) * (BM / WR), wn = (wave % WC) * (BN / WC);
+  v16f acc[RA][RB];
+#pragma unroll
+  for (int i = 0; i < RA; ++i)
+#pragma unroll
+    for (int j = 0; j < RB; ++j) acc[i][j] = 0.f;
+  auto load = [&](int s) {
+    const int l = (int)std::min<int64_t>(left - (int64_t)s * kBK, kBK);
+    a.load(&lds[s & 1][0], wave, l);
+    b.load(&lds[s & 1][BM * 128], wave, l);
+  };
+  if (steps > 0) load(0);
+  for (int s = 0; s < steps; ++s) {
+    wait_vm<0>();
+    __syncthreads();  // step s has landed everywhere, step s - 1 is read
+    if (s + 1 < steps) load(s + 1);
+    const uint8_t *la = &lds[s & 1][0], *lb = &lds[s & 1][BM * 128];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      v4i fa[RA], fb[RB];
+#pragma unroll
+      for (int i = 0; i < RA; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, kk, lane);
+#pragma unroll
+      for (int j = 0; j < RB; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, kk, lane);
+#pragma unroll
+      for (int i = 0; i < RA; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
+    }
+  }
+  // Lane (j, g) holds column j and rows (r & 3) + 8 (r >> 2) + 4 g of each 32 x 32.
+  // 32 rows of the wave's columns at a time go through LDS, so that the epilogue
+  // loads, computes and stores whole pieces of rows.
+  constexpr int kCols = BN / WC, kLanes = kCols / Piece<E>::n, kRows = 64 / kLanes;
+  const int j = lane & 31, g = lane >> 5, c = lane % kLanes * Piece<E>::n;
+  const int N = (int)p.N, col = (int)n0 + wn + c;
+  float bias[Piece<E>::n];
+  bias_piece<E>(p.epi, col, N, bias);
+  __syncthreads();  // the last step is read
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * kCols;
+#pragma unroll
+  for (int ii = 0; ii < RA; ++ii) {
+#pragma unroll
+    for (int jj = 0; jj < RB; ++jj)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) strip[((r & 3) + 8 * (r >> 2) + 4 * g) * kCols + 32 * jj + j] = acc[ii][jj][r];
+#pragma unroll 1
+    for (int q = 0; q < 32; q += kRows) {
+      const int64_t row = m0 + wm + 32 * ii + q + lane / kLanes;
+      const typename Piece<E>::fvec z =
+          *reinterpret_cast<const typename Piece<E>::fvec*>(strip + (q + lane / kLanes) * kCols + c);
+      if (row >= p.M || col >= N) continue;
+      if (p.part) {
+        float* d = p.part + ((int64_t)split * p.M + row) * N;
+#pragma unroll
+        for (int e = 0; e < Piece<E>::n; e += 4)
+          if (col + e < N) store_piece<float>(d, col + e, N, Piece<float>::vec{z[e], z[e + 1], z[e + 2], z[e + 3]});
+      } else {
+        finish_piece<E>(p.epi, z, bias, row, col, N);
+      }
+    }
+  }
+}
+
+// The splits' sums added in order, then the epilogue.
+template <class E>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t M, int N,
+                                                   Epilogue epi) {
+  constexpr int n = Piece<E>::n;
+  const int per_row = (N + n - 1) / n;
+  const int64_t total = M * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / per_row;
+    const int c = (int)(i - m * per_row) * n;
+    typename Piece<E>::fvec z = 0.f;
+    for (int k = 0; k < splits; ++k) {
+      float f[n];
+      load_params(f, part + ((int64_t)k * M + m) * N, c, N, 0.f);
+#pragma unroll
+      for (int e = 0; e < n; ++e) z[e] += f[e];
+    }
+    float bias[n];
+    bias_piece<E>(epi, c, N, bias);
+    finish_piece<E>(epi, z, bias, m, c, N);
+  }
+}
+
+// ---- few tokens -------------------------------------------------------------
+
+// Up to 16 MT tokens: bound by reading W once.  A workgroup of NW waves takes 16
+// rows of W, each wave a share of K straight from memory into fragments (no LDS:
+// nothing of W is used twice), any alignment; the waves' sums are added in order.
+template <class E, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void few_kernel(const E* __restrict__ x, int64_t ldx, const E* __restrict__ w,
+                                                      int64_t ldw, int M, int64_t N, int K, Epilogue epi) {
+  constexpr int kPer = Piece<E>::n, kStep = 4 * kPer;  // 64 bytes of a row: a chunk each for 4 lanes
+  constexpr int kAhead = 4;
+  typedef typename Piece<E>::vec V;
+  __shared__ v4f sum[NW][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  // Rows past the end repeat the last one; their sums are not stored.
+  const E* wr = w + std::min<int64_t>(n0 + i, N - 1) * ldw + g * kPer;
+  const E* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = x + (int64_t)min(16 * t + i, M - 1) * ldx + g * kPer;
+  v4f acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = 0.f;
+  auto multiply = [&](V wv, V xv, v4f c) {
+    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[s], wv[s], c, 0, 0, 0);
+      return c;
+    } else if constexpr (std::is_same_v<E, __bf16>) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, wv, c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(xv, wv, c, 0, 0, 0);
+    }
+  };
+  typedef typename Piece<E>::any Any;
+  // Whole steps: the waves take groups of kAhead in turn.
+  const int steps = K / kStep, groups = steps / kAhead;
+  for (int q = wave; q < groups; q += NW) {
+    const int k0 = q * kAhead * kStep;
+    V wv[kAhead], xv[kAhead][MT];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      wv[u] = *reinterpret_cast<const Any*>(wr + k0 + u * kStep);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xv[u][t] = *reinterpret_cast<const Any*>(xr[t] + k0 + u * kStep);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = multiply(wv[u], xv[u][t], acc[t]);
+  }
+  // The rest, a step a wave; past K both operands are zero.
+  for (int q = groups * kAhead + wave; q * kStep < K; q += NW) {
+    const int k0 = q * kStep;
+    const V wv = load_piece(wr - g * kPer, k0 + g * kPer, K);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = multiply(wv, load_piece(xr[t] - g * kPer, k0 + g * kPer, K), acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) sum[wave][t][lane] = acc[t];
+  __syncthreads();
+  // Lane (i, g) of a sum holds column n0 + i and tokens 4 g .. 4 g + 3.
+  for (int q = threadIdx.x; q < MT * 64; q += 64 * NW) {
+    const int t = q >> 6, l = q & 63;
+    v4f s = sum[0][t][l];
+#pragma unroll
+    for (int v = 1; v < NW; ++v) s += sum[v][t][l];
+    const int64_t n = n0 + (l & 15);
+    if (n >= N) continue;
+    const float bias = bias_at<E>(epi, n);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = 16 * t + 4 * (l >> 4) + r;
+      if (m < M) finish<E>(epi, s[r], bias, m, n, N);
+    }
+  }
+}
+
+// ---- dZ and db ----------------------------------------------------------------
+
+// dz = dy act'(z) (unless dz is null), zero from N to ldz's next whole piece, and
+// this workgroup's column sums in part[blockIdx.y][N] (unless part is null).  64
+// pieces of columns, 4 rows at a time.
+template <class E>
+__global__ __launch_bounds__(256) void slope_kernel(const E* __restrict__ dy, int64_t lddy,
+                                                    const typename Slope<E>::type* __restrict__ slope, int64_t M, int N,
+                                                    E* __restrict__ dz, int64_t ldz, float* __restrict__ part) {
+  constexpr int n = Piece<E>::n;
+  typedef typename Piece<E>::vec V;
+  typedef typename Piece<E>::fvec F;
+  typedef typename Slope<E>::type S;
+  typedef S SV __attribute__((ext_vector_type(16 / sizeof(E))));
+  typedef SV SAny __attribute__((aligned(sizeof(S))));
+  __shared__ float sum[4][64 * n];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c64 = ((int64_t)blockIdx.x * 64 + lane) * n;
+  F s = 0.f;
+  if (c64 < N) {
+    const int c = (int)c64;
+    for (int64_t row = (int64_t)blockIdx.y * 4 + wave; row < M; row += (int64_t)gridDim.y * 4) {
+      F f = __builtin_convertvector(load_piece(dy + row * lddy, c, N), F);
+      if (slope) {
+        const S* sr = slope + row * N + c;
+        if (c + n <= N) {
+          const SV v = *reinterpret_cast<const SAny*>(sr);
+#pragma unroll
+          for (int e = 0; e < n; ++e) f[e] *= Slope<E>::unpack(v[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < n; ++e) f[e] = c + e < N ? f[e] * Slope<E>::unpack(sr[e]) : 0.f;
+        }
+        if (dz) *reinterpret_cast<V*>(dz + row * ldz + c) = __builtin_convertvector(f, V);
+      }
+      s += f;
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < n; ++e) sum[wave][lane * n + e] = s[e];
+  __syncthreads();
+  for (int j = threadIdx.x; j < 64 * n; j += 256) {
+    const int64_t col = (int64_t)blockIdx.x * 64 * n + j;
+    if (col < N) part[(int64_t)blockIdx.y * N + col] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
+  }
+}
+
+template <class W>
+__global__ __launch_bounds__(256) void bias_sum_kernel(const float* __restrict__ part, int n, int N, W* __restrict__ db) {
+  __shared__ float sum[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < N)
+    for (int k = wave; k < n; k += 4) s += part[(int64_t)k * N + c];
+  sum[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < N) db[c] = (W)((sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]));
+}
+
+// ---- host ---------------------------------------------------------------------
+
+constexpr int kCus = 256;
+
+int launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? VOID_OK : void_internal_fail(VOID_ERR_HIP, hipGetErrorString(e));
+}
+
+bool float_type(int32_t t) { return t == VOID_DT_F32 || t == VOID_DT_BF16 || t == VOID_DT_F16; }
+int size_of(int32_t t) { return t == VOID_DT_F32 ? 4 : 2; }
+
+template <class Go>
+void by_type(int32_t dtype, Go go) {
+  if (dtype == VOID_DT_F32) go(float{});
+  else if (dtype == VOID_DT_BF16) go(__bf16{});
+  else go(_Float16{});
+}
+
+// A tile size and the K splits of a product.
+struct Plan {
+  int tile, splits, steps_per_split;
+};
+
+Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
+  const int64_t steps = std::max<int64_t>(1, (K * esz + 127) / 128);
+  Plan best{128, 1, (int)steps};
+  double least = 1e300;
+  for (int tile : {256, 128}) {
+    const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+    const int64_t slots = kCus * (tile == 256 ? 1 : 2);
+    for (int splits = 1; splits <= 16 && splits <= steps; ++splits) {
+      const int64_t per = (steps + splits - 1) / splits;
+      if (splits > 1 && ((steps + per - 1) / per != splits || per < 4)) continue;
+      const int64_t rounds = (tiles * splits + slots - 1) / slots;
+      // Microseconds: a step of a full round, and the partial sums' traffic.
+      const double step = esz == 4 ? (tile == 256 ? 7.2 : 3.7) : (tile == 256 ? 0.95 : 0.65);
+      const double cost = rounds * (per * step + 3.0) + (splits > 1 ? 4.0 + 8.0 * splits * M * N / 4e6 : 0.0);
+      if (cost < least) {
+        least = cost;
+        best = Plan{tile, splits, (int)per};
+      }
+    }
+  }
+  return best;
+}
+
+template <class E, bool TA, bool TB>
+void product(Product p, const Plan& plan, hipStream_t stream) {
+  p.splits = plan.splits;
+  p.steps_per_split = plan.steps_per_split;
+  p.tiles_m = (int)((p.M + plan.tile - 1) / plan.tile);
+  p.tiles_n = (int)((p.N + plan.tile - 1) / plan.tile);
+  const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * plan.splits));
+  if (plan.tile == 256) hipLaunchKernelGGL((product_kernel<E, 256, 256, 2, 4, TA, TB>), grid, dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((product_kernel<E, 128, 128, 2, 2, TA, TB>), grid, dim3(256), 0, stream, p);
+  if (plan.splits > 1)
+    hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)std::min<int64_t>((p.M * ((p.N * (int64_t)sizeof(E) + 15) / 16) + 255) / 256, kCus * 16)),
+                       dim3(256), 0, stream, p.part, plan.splits, p.M, (int)p.N, p.epi);
+}
+
+template <class E>
+void few(const void_linear_args* d, const Epilogue& epi, hipStream_t stream) {
+  auto go = [&](auto mt, auto nw) {
+    constexpr int MT = decltype(mt)::value, NW = decltype(nw)::value;
+    hipLaunchKernelGGL((few_kernel<E, MT, NW>), dim3((unsigned)((d->N + 15) / 16)), dim3(64 * NW), 0, stream,
+                       static_cast<const E*>(d->x), d->ldx, static_cast<const E*>(d->w), d->ldw, (int)d->M, d->N,
+                       (int)d->K, epi);
+  };
+  auto waves = [&](auto mt) {
+    if (d->N >= 8192) go(mt, std::integral_constant<int, 4>{});
+    else go(mt, std::integral_constant<int, 16>{});
+  };
+  if (d->M <= 16) waves(std::integral_constant<int, 1>{});
+  else if (d->M <= 32) waves(std::integral_constant<int, 2>{});
+  else waves(std::integral_constant<int, 4>{});
+}
+
+bool few_tokens(int64_t M) { return M <= 64; }
+
+// Rows that the LDS-DMA reads in whole chunks: aligned, of whole chunks.
+bool whole_chunks(const void* p, int64_t ld, int64_t cols, int esz) {
+  return (uintptr_t)p % 16 == 0 && ld * esz % 16 == 0 && cols * esz % 16 == 0;
+}
+
+int check(const void_linear_args* d) {
+  if (!d) return void_internal_fail(VOID_ERR_ARG, "null arguments");
+  if (d->M < 0 || d->N < 0 || d->K < 0) return void_internal_fail(VOID_ERR_ARG, "negative size");
+  if (d->N > INT_MAX / 2 || d->K > INT_MAX / 2 || d->M > INT_MAX)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "sizes are limited to 2^30 features and 2^31 rows");
+  if (!float_type(d->dtype)) return void_internal_fail(VOID_ERR_UNSUPPORTED, "values are fp32, bf16 or fp16");
+  return 1;
+}
+
+int64_t padded(int64_t cols, int esz) { return (cols * esz + 15) / 16 * 16 / esz; }
+
+}  // namespace
+
+extern "C" {
+
+int32_t void_linear_any_alignment(int64_t M) { return few_tokens(M); }
+
+size_t void_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+  if (M <= 0 || N <= 0 || few_tokens(M)) return 0;
+  const Plan p = plan_of(M, N, K, size_of(dtype));
+  return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
+}
+
+int void_linear(const void_linear_args* d, hipStream_t stream) {
+  void_internal_fail(VOID_OK, "");
+  const int st = check(d);
+  if (st <= 0) return st;
+  if (d->M == 0 || d->N == 0) return VOID_OK;
+  const int esz = size_of(d->dtype);
+  if (!d->y || (d->K && (!d->x || !d->w))) return void_internal_fail(VOID_ERR_ARG, "null x, w or y");
+  if (d->bias && d->bias_dtype != d->dtype && d->bias_dtype != VOID_DT_F32)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "the bias has the values' type, or fp32");
+  if (d->activation < VOID_ACT_NONE || d->activation > VOID_ACT_SILU)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "unknown activation");
+  if (d->slope && d->activation == VOID_ACT_NONE) return void_internal_fail(VOID_ERR_ARG, "slope without an activation");
+  if ((d->M > 1 && (d->ldx < d->K || d->ldy < d->N || (d->residual && d->ldr < 0))) || (d->N > 1 && d->ldw < d->K))
+    return void_internal_fail(VOID_ERR_ARG, "leading dimension too small");
+  if (((uintptr_t)d->x | (uintptr_t)d->w | (uintptr_t)d->y | (uintptr_t)d->residual | (uintptr_t)d->slope) % esz ||
+      (d->bias && (uintptr_t)d->bias % size_of(d->bias_dtype)))
+    return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
+  const Epilogue epi{d->y, d->ldy, d->bias, d->residual, d->ldr, d->slope, d->bias_dtype == VOID_DT_F32, d->activation};
+  if (few_tokens(d->M)) {
+    by_type(d->dtype, [&](auto e) { few<decltype(e)>(d, epi, stream); });
+    return launched();
+  }
+  if (d->K && (!whole_chunks(d->x, d->ldx, d->K, esz) || !whole_chunks(d->w, d->ldw, d->K, esz)))
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "more than 64 tokens need rows of whole 16-byte chunks");
+  if (256 * std::max(d->ldx, d->ldw) * esz > INT_MAX - 65536)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
+  const Plan plan = plan_of(d->M, d->N, d->K, esz);
+  if (plan.splits > 1 && (!d->workspace || (uintptr_t)d->workspace % 4 ||
+                          d->workspace_bytes < (size_t)plan.splits * d->M * d->N * 4))
+    return void_internal_fail(VOID_ERR_WORKSPACE, "linear: workspace missing or too small");
+  by_type(d->dtype, [&](auto e) {
+    product<decltype(e), false, false>(Product{d->x, d->w, d->ldx, d->ldw, d->M, d->N, d->K, 0, 0, 0, 0,
+                                               plan.splits > 1 ? static_cast<float*>(d->workspace) : nullptr, epi},
+                                       plan, stream);
+  });
+  return launched();
+}
+
+int void_linear_grad_x(const void* dz, int64_t ldz, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K,
+                       int32_t dtype, void* dx, int64_t ldx, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream) {
+  void_internal_fail(VOID_OK, "");
+  const void_linear_args d{.M = M, .N = N, .K = K, .dtype = dtype};
+  const int st = check(&d);
+  if (st <= 0) return st;
+  if (M == 0 || K == 0) return VOID_OK;
+  const int esz = size_of(dtype);
+  if (!dx || (N && (!dz || !w))) return void_internal_fail(VOID_ERR_ARG, "null array");
+  if (M > 1 && (ldz < N || ldx < K)) return void_internal_fail(VOID_ERR_ARG, "leading dimension too small");
+  if ((uintptr_t)dx % esz) return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
+  if (N && (!whole_chunks(dz, ldz, padded(N, esz), esz) || ldz < padded(N, esz) ||
+            !whole_chunks(w, ldw, padded(K, esz), esz) || ldw < padded(K, esz)))
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "the products of the gradient need rows of whole 16-byte chunks");
+  if (256 * std::max(ldz, ldw) * esz > INT_MAX - 65536)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
+  const Plan plan = plan_of(M, K, N, esz);
+  if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)plan.splits * M * K * 4))
+    return void_internal_fail(VOID_ERR_WORKSPACE, "linear gradient: workspace missing or too small");
+  by_type(dtype, [&](auto e) {
+    product<decltype(e), false, true>(Product{dz, w, ldz, ldw, M, K, N, 0, 0, 0, 0,
+                                              plan.splits > 1 ? static_cast<float*>(workspace) : nullptr,
+                                              Epilogue{dx, ldx, nullptr, nullptr, 0, nullptr, 0, VOID_ACT_NONE}},
+                                      plan, stream);
+  });
+  return launched();
+}
+
+int void_linear_grad_w(const void* dz, int64_t ldz, const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K,
+                       int32_t dtype, void* dw, int64_t ldw, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream) {
+  void_internal_fail(VOID_OK, "");
+  const void_linear_args d{.M = M, .N = N, .K = K, .dtype = dtype};
+  const int st = check(&d);
+  if (st <= 0) return st;
+  if (N == 0 || K == 0) return VOID_OK;
+  const int esz = size_of(dtype);
+  if (!dw || (M && (!dz || !x))) return void_internal_fail(VOID_ERR_ARG, "null array");
+  if (N > 1 && ldw < K) return void_internal_fail(VOID_ERR_ARG, "leading dimension too small");
+  if ((uintptr_t)dw % esz) return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
+  if (M && (!whole_chunks(dz, ldz, padded(N, esz), esz) || ldz < padded(N, esz) ||
+            !whole_chunks(x, ldx, padded(K, esz), esz) || ldx < padded(K, esz)))
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "the products of the gradient need rows of whole 16-byte chunks");
+  if (256 * std::max(ldz, ldx) * esz > INT_MAX - 65536)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
+  const Plan plan = plan_of(N, K, M, esz);
+  if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)plan.splits * N * K * 4))
+    return void_internal_fail(VOID_ERR_WORKSPACE, "linear gradient: workspace missing or too small");
+  by_type(dtype, [&](auto e) {
+    product<decltype(e), true, true>(Product{dz, x, ldz, ldx, N, K, M, 0, 0, 0, 0,
+                                             plan.splits > 1 ? static_cast<float*>(workspace) : nullptr,
+                                             Epilogue{dw, ldw, nullptr, nullptr, 0, nullptr, 0, VOID_ACT_NONE}},
+                                     plan, stream);
+  });
+  return launched();
+}
+
+size_t void_linear_grad_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t dtype) {
+  if (rows <= 0 || cols <= 0) return 0;
+  const Plan p = plan_of(rows, cols, depth, size_of(dtype));
+  return p.splits > 1 ? (size_t)p.splits * rows * cols * 4 : 0;
+}
+
+static int slope_grid(int64_t M, int64_t N, int32_t dtype) {
+  const int64_t gx = (N * size_of(dtype) + 1023) / 1024;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((M + 3) / 4, (kCus * 8 + gx - 1) / gx));
+}
+
+size_t void_linear_grad_z_workspace_bytes(int64_t M, int64_t N, int32_t dtype) {
+  return M <= 0 || N <= 0 ? 0 : (size_t)slope_grid(M, N, dtype) * N * 4;
+}
+
+int void_linear_grad_z(const void* dy, int64_t lddy, const void* slope, int64_t M, int64_t N, int32_t dtype, void* dz,
+                       int64_t ldz, void* db, int32_t bias_dtype, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream) {
+  void_internal_fail(VOID_OK, "");
+  const void_linear_args d{.M = M, .N = N, .dtype = dtype};
+  const int st = check(&d);
+  if (st <= 0) return st;
+  if (N == 0 || (!dz && !db)) return VOID_OK;
+  const int esz = size_of(dtype);
+  if (M && !dy) return void_internal_fail(VOID_ERR_ARG, "null dy");
+  if (dz && (!slope || (uintptr_t)dz % 16 || ldz * esz % 16 || ldz < padded(N, esz)))
+    return void_internal_fail(VOID_ERR_ARG, "dz needs the slope and rows of whole 16-byte chunks");
+  if (db && bias_dtype != dtype && bias_dtype != VOID_DT_F32)
+    return void_internal_fail(VOID_ERR_UNSUPPORTED, "the bias has the values' type, or fp32");
+  if (((uintptr_t)dy | (uintptr_t)slope) % esz || (uintptr_t)db % size_of(bias_dtype) || (M > 1 && lddy < 0))
+    return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
+  const int gy = M ? slope_grid(M, N, dtype) : 0;
+  if (db && M && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)gy * N * 4))
+    return void_internal_fail(VOID_ERR_WORKSPACE, "linear gradient: workspace missing or too small");
+  by_type(dtype, [&](auto e) {
+    using E = decltype(e);
+    if (M)
+      hipLaunchKernelGGL(slope_kernel<E>, dim3((unsigned)((N * esz + 1023) / 1024), gy), dim3(256), 0, stream,
+                         static_cast<const E*>(dy), lddy, static_cast<const typename Slope<E>::type*>(slope), M, (int)N,
+                         static_cast<E*>(dz), ldz, db ? static_cast<float*>(workspace) : nullptr);
+    if (db) {
+      const dim3 grid((unsigned)((N + 63) / 64));
+      if (bias_dtype == VOID_DT_F32)
+        hipLaunchKernelGGL(bias_sum_kernel<float>, grid, dim3(256), 0, stream, static_cast<float*>(workspace), gy,
+                           (int)N, static_cast<float*>(db));
+      else
+        hipLaunchKernelGGL(bias_sum_kernel<E>, grid, dim3(256), 0, stream, static_cast<float*>(workspace), gy, (int)N,
+                           static_cast<E*>(db));
+    }
+  });
+  return launched();
+}
+
+}  // extern "C"
