@@ -208,12 +208,14 @@ struct Operand {
     }
   }
 
-  // The next step into LDS; `left` values of r remain from it on.
+  // Loads [F, T) of the next step into LDS, the last of them stepping on; `left`
+  // values of r remain from it on.
+  template <int F = 0, int T = kLoads>
   __device__ __forceinline__ void load(uint8_t* lds, int wave, int left) {
     const v4s r = sgpr_rsrc(base);
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) dma_b128(r, lds + (q * NW + wave) * 1024, at[q] < left ? voff[q] : kOutOfRange, 0);
-    base += step;
+    for (int q = F; q < T; ++q) dma_b128(r, lds + (q * NW + wave) * 1024, at[q] < left ? voff[q] : kOutOfRange, 0);
+    if (F < T && T == kLoads) base += step;
   }
 
   // Chunk pair kk's fragment of rows i0 .. i0 + 31: 16 bytes along r a lane.
@@ -245,92 +247,216 @@ struct Operand {
   }
 };
 
-template <class E, int BM, int BN, int WR, int WC, bool TA, bool TB>
-__global__ __launch_bounds__(64 * WR * WC) void product_kernel(Product p) {
-  constexpr int NW = WR * WC, kBK = 128 / (int)sizeof(E), RA = BM / WR / 32, RB = BN / WC / 32;
-  typedef Operand<E, BM, NW, TA> OpA;
-  typedef Operand<E, BN, NW, TB> OpB;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][(BM + BN) * 128];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups are dealt to the 8 XCDs in turn: each XCD gets a run of
-  // neighbouring tiles, whose operands its L2 then holds.
-  const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3;
-  int t = x * q + min(x, n & 7) + (blockIdx.x >> 3);
-  const int tiles = p.tiles_m * p.tiles_n, split = t / tiles;
-  t -= split * tiles;
-  constexpr int kGroup = 4;
-  const int group = t / (kGroup * p.tiles_n), first = group * kGroup, size = min(kGroup, p.tiles_m - first);
-  const int in = t - group * kGroup * p.tiles_n;
-  const int64_t m0 = (int64_t)(first + in % size) * BM, n0 = (int64_t)(in / size) * BN;
+// Which tile and split of the grid a workgroup takes.  Workgroups are dealt to the
+// 8 XCDs in turn: each XCD gets a run of neighbouring tiles, whose operands its L2
+// then holds.
+template <int BM, int BN>
+struct Place {
+  int64_t m0, n0, r0, left;  // first row and column, first r and how many of them
+  int split;
+  __device__ __forceinline__ Place(const Product& p, int bk) {
+    const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3;
+    int t = x * q + min(x, n & 7) + (blockIdx.x >> 3);
+    const int tiles = p.tiles_m * p.tiles_n;
+    split = t / tiles;
+    t -= split * tiles;
+    constexpr int kGroup = 4;
+    const int group = t / (kGroup * p.tiles_n), first = group * kGroup, size = min(kGroup, p.tiles_m - first);
+    const int in = t - group * kGroup * p.tiles_n;
+    m0 = (int64_t)(first + in % size) * BM;
+    n0 = (int64_t)(in / size) * BN;
+    r0 = (int64_t)split * p.steps_per_split * bk;
+    left = std::min<int64_t>(p.K - r0, (int64_t)p.steps_per_split * bk);
+  }
+};
 
-  const int64_t r0 = (int64_t)split * p.steps_per_split * kBK;
-  const int64_t left = std::min<int64_t>(p.K - r0, (int64_t)p.steps_per_split * kBK);
-  const int steps = (int)((left + kBK - 1) / kBK);
+// 32 rows x COLS columns of sums from the wave's strip in LDS: whole pieces of
+// rows through the epilogue (or to the partial sums).
+template <class E, int COLS>
+__device__ __forceinline__ void store_strip(const Product& p, int split, const float* strip, int64_t row0, int64_t col0,
+                                            int lane) {
+  constexpr int kLanes = COLS / Piece<E>::n, kRows = 64 / kLanes;
+  const int c = lane % kLanes * Piece<E>::n, N = (int)p.N, col = (int)col0 + c;
+  float bias[Piece<E>::n];
+  bias_piece<E>(p.epi, col, N, bias);
+#pragma unroll 1
+  for (int q = lane / kLanes; q < 32; q += kRows) {
+    const int64_t row = row0 + q;
+    const typename Piece<E>::fvec z = *reinterpret_cast<const typename Piece<E>::fvec*>(strip + q * COLS + c);
+    if (row >= p.M || col >= N) continue;
+    if (p.part) {
+      float* d = p.part + ((int64_t)split * p.M + row) * N;
+#pragma unroll
+      for (int e = 0; e < Piece<E>::n; e += 4)
+        if (col + e < N) store_piece<float>(d, col + e, N, Piece<float>::vec{z[e], z[e + 1], z[e + 2], z[e + 3]});
+    } else {
+      finish_piece<E>(p.epi, z, bias, row, col, N);
+    }
+  }
+}
+
+// A 32 x 32 block of sums into a strip: lane (j, g) holds column j and rows
+// (r & 3) + 8 (r >> 2) + 4 g.
+template <int COLS>
+__device__ __forceinline__ void to_strip(float* strip, int col, v16f acc, int lane) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) strip[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * COLS + col + (lane & 31)] = acc[r];
+}
+
+// 128 x 128 tiles, 4 waves of 64 x 64, two steps in LDS, two workgroups a CU.
+template <class E, bool TA, bool TB>
+__global__ __launch_bounds__(256) void product_kernel(Product p) {
+  constexpr int B = 128, NW = 4, kBK = 128 / (int)sizeof(E), R = 2;
+  typedef Operand<E, B, NW, TA> OpA;
+  typedef Operand<E, B, NW, TB> OpB;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2 * B * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place<B, B> at(p, kBK);
+  const int steps = (int)((at.left + kBK - 1) / kBK);
   OpA a;
   OpB b;
-  a.init(p.a, p.lda, m0, p.M, r0, wave, lane);
-  b.init(p.b, p.ldb, n0, p.N, r0, wave, lane);
-  const int wm = (wave / WC) * (BM / WR), wn = (wave % WC) * (BN / WC);
-  v16f acc[RA][RB];
+  a.init(p.a, p.lda, at.m0, p.M, at.r0, wave, lane);
+  b.init(p.b, p.ldb, at.n0, p.N, at.r0, wave, lane);
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  v16f acc[R][R];
 #pragma unroll
-  for (int i = 0; i < RA; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < RB; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
   auto load = [&](int s) {
-    const int l = (int)std::min<int64_t>(left - (int64_t)s * kBK, kBK);
+    const int l = (int)std::min<int64_t>(at.left - (int64_t)s * kBK, kBK);
     a.load(&lds[s & 1][0], wave, l);
-    b.load(&lds[s & 1][BM * 128], wave, l);
+    b.load(&lds[s & 1][B * 128], wave, l);
   };
   if (steps > 0) load(0);
   for (int s = 0; s < steps; ++s) {
     wait_vm<0>();
     __syncthreads();  // step s has landed everywhere, step s - 1 is read
     if (s + 1 < steps) load(s + 1);
-    const uint8_t *la = &lds[s & 1][0], *lb = &lds[s & 1][BM * 128];
+    const uint8_t *la = &lds[s & 1][0], *lb = &lds[s & 1][B * 128];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      v4i fa[RA], fb[RB];
+      v4i fa[R], fb[R];
 #pragma unroll
-      for (int i = 0; i < RA; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, kk, lane);
+      for (int i = 0; i < R; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, kk, lane);
 #pragma unroll
-      for (int j = 0; j < RB; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, kk, lane);
+      for (int j = 0; j < R; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, kk, lane);
 #pragma unroll
-      for (int i = 0; i < RA; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < RB; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
+        for (int j = 0; j < R; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
     }
   }
-  // Lane (j, g) holds column j and rows (r & 3) + 8 (r >> 2) + 4 g of each 32 x 32.
-  // 32 rows of the wave's columns at a time go through LDS, so that the epilogue
-  // loads, computes and stores whole pieces of rows.
-  constexpr int kCols = BN / WC, kLanes = kCols / Piece<E>::n, kRows = 64 / kLanes;
-  const int j = lane & 31, g = lane >> 5, c = lane % kLanes * Piece<E>::n;
-  const int N = (int)p.N, col = (int)n0 + wn + c;
-  float bias[Piece<E>::n];
-  bias_piece<E>(p.epi, col, N, bias);
   __syncthreads();  // the last step is read
-  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * kCols;
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * 64;
 #pragma unroll
-  for (int ii = 0; ii < RA; ++ii) {
+  for (int i = 0; i < R; ++i) {
 #pragma unroll
-    for (int jj = 0; jj < RB; ++jj)
+    for (int j = 0; j < R; ++j) to_strip<64>(strip, 32 * j, acc[i][j], lane);
+    store_strip<E, 64>(p, at.split, strip, at.m0 + wm + 32 * i, at.n0 + wn, lane);
+  }
+}
+
+// 256 x 256 tiles of 16-bit operands, 4 waves of 128 x 128, one workgroup a CU: the
+// fewest LDS bytes a product (a wave's fragments serve 16 matrix instructions from 8
+// reads), with 256 accumulators a lane.
+//
+// A step (64 of r) is four fragment sets; each set is read while the matrix cores
+// work on the one before it, across the steps too: the one barrier of a step stands
+// before its last set, when all of the step has been read and the next step has
+// landed.  LDS holds three steps of A and two of B (all 160 KB): the loads of a step
+// are spread over the sets, four each, so that no wave waits to issue them, and the
+// waits count those of A for the step after next, which stay in flight.
+template <class E, bool TA, bool TB>
+__global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
+  constexpr int B = 256, NW = 4, kBK = 64, R = 4, kOperand = B * 128;
+  typedef Operand<E, B, NW, TA> OpA;
+  typedef Operand<E, B, NW, TB> OpB;
+  static_assert(OpA::kLoads == 8 && OpB::kLoads == 8);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[5][kOperand];  // A: 0 1 2, B: 3 4
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place<B, B> at(p, kBK);
+  const int steps = (int)((at.left + kBK - 1) / kBK);
+  OpA a;
+  OpB b;
+  a.init(p.a, p.lda, at.m0, p.M, at.r0, wave, lane);
+  b.init(p.b, p.ldb, at.n0, p.N, at.r0, wave, lane);
+  const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
+  v16f acc[R][R];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) strip[((r & 3) + 8 * (r >> 2) + 4 * g) * kCols + 32 * jj + j] = acc[ii][jj][r];
-#pragma unroll 1
-    for (int q = 0; q < 32; q += kRows) {
-      const int64_t row = m0 + wm + 32 * ii + q + lane / kLanes;
-      const typename Piece<E>::fvec z =
-          *reinterpret_cast<const typename Piece<E>::fvec*>(strip + (q + lane / kLanes) * kCols + c);
-      if (row >= p.M || col >= N) continue;
-      if (p.part) {
-        float* d = p.part + ((int64_t)split * p.M + row) * N;
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int e = 0; e < Piece<E>::n; e += 4)
-          if (col + e < N) store_piece<float>(d, col + e, N, Piece<float>::vec{z[e], z[e + 1], z[e + 2], z[e + 3]});
-      } else {
-        finish_piece<E>(p.epi, z, bias, row, col, N);
-      }
+    for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+  // What is left of r at step s; past the last step nothing: such loads bring zeros
+  // and ask for no memory.
+  auto left = [&](int s) { return (int)std::max<int64_t>(0, std::min<int64_t>(at.left - (int64_t)s * kBK, kBK)); };
+  v4i fa[2][R], fb[2][R];
+  // Where A of this step, the next and the one after next are, and B of this and the next.
+  const uint8_t *a0 = lds[0], *a1 = lds[1], *a2 = lds[2], *b0 = lds[3], *b1 = lds[4];
+  // Set kk's products, two at a time behind one of the next set's eight reads and,
+  // every second time, one of the phase's four loads.  The reads come in the order in
+  // which the next set's products take them.
+  auto phase = [&](auto kk_, const uint8_t* ra, const uint8_t* rb, auto load) {
+    constexpr int kk = decltype(kk_)::value, next = (kk + 1) & 3, set = kk & 1, to = next & 1;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (q == 0) fb[to][0] = OpB::fragment(rb, wn, next, lane);
+      if (q == 1) fa[to][0] = OpA::fragment(ra, wm, next, lane);
+      if (q >= 2 && q <= 4) fb[to][q - 1] = OpB::fragment(rb, wn + 32 * (q - 1), next, lane);
+      if (q >= 5) fa[to][q - 4] = OpA::fragment(ra, wm + 32 * (q - 4), next, lane);
+      if (q == 0) load(std::integral_constant<int, 0>{});
+      if (q == 2) load(std::integral_constant<int, 1>{});
+      if (q == 4) load(std::integral_constant<int, 2>{});
+      if (q == 6) load(std::integral_constant<int, 3>{});
+      const int i = q >> 1, j = (q & 1) * 2;
+      acc[i][j] = mfma(fa[set][i], fb[set][j], acc[i][j], E{});
+      acc[i][j + 1] = mfma(fa[set][i], fb[set][j + 1], acc[i][j + 1], E{});
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  a.load(const_cast<uint8_t*>(a0), wave, left(0));
+  b.load(const_cast<uint8_t*>(b0), wave, left(0));
+  a.load(const_cast<uint8_t*>(a1), wave, left(1));
+  b.template load<0, 4>(const_cast<uint8_t*>(b1), wave, left(1));
+  wait_vm<12>();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    fb[0][i] = OpB::fragment(b0, wn + 32 * i, 0, lane);
+    fa[0][i] = OpA::fragment(a0, wm + 32 * i, 0, lane);
+  }
+  for (int s = 0; s < steps; ++s) {
+    const int l1 = left(s + 1), l2 = left(s + 2);
+    phase(std::integral_constant<int, 0>{}, a0, b0, [&](auto q) {
+      constexpr int n = 4 + decltype(q)::value;
+      b.template load<n, n + 1>(const_cast<uint8_t*>(b1), wave, l1);
+    });
+    phase(std::integral_constant<int, 1>{}, a0, b0, [&](auto q) {
+      constexpr int n = decltype(q)::value;
+      a.template load<n, n + 1>(const_cast<uint8_t*>(a2), wave, l2);
+    });
+    phase(std::integral_constant<int, 2>{}, a0, b0, [&](auto q) {
+      constexpr int n = 4 + decltype(q)::value;
+      a.template load<n, n + 1>(const_cast<uint8_t*>(a2), wave, l2);
+    });
+    wait_vm<8>();     // A of step s + 2 stays in flight
+    __syncthreads();  // step s is read, step s + 1 has landed
+    phase(std::integral_constant<int, 3>{}, a1, b1, [&](auto q) {
+      constexpr int n = decltype(q)::value;
+      b.template load<n, n + 1>(const_cast<uint8_t*>(b0), wave, l2);
+    });
+    const uint8_t *a3 = a0, *b2 = b0;
+    a0 = a1, a1 = a2, a2 = a3;
+    b0 = b1, b1 = b2;
+  }
+  wait_vm<0>();     // loads past the last step still write zeros
+  __syncthreads();
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * 128;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) to_strip<128>(strip, 32 * j, acc[i][j], lane);
+    store_strip<E, 128>(p, at.split, strip, at.m0 + wm + 32 * i, at.n0 + wn, lane);
   }
 }
 
@@ -525,6 +651,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
   Plan best{128, 1, (int)steps};
   double least = 1e300;
   for (int tile : {256, 128}) {
+    if (tile == 256 && esz == 4) continue;
     const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
     const int64_t slots = kCus * (tile == 256 ? 1 : 2);
     for (int splits = 1; splits <= 16 && splits <= steps; ++splits) {
@@ -532,7 +659,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
       if (splits > 1 && ((steps + per - 1) / per != splits || per < 4)) continue;
       const int64_t rounds = (tiles * splits + slots - 1) / slots;
       // Microseconds: a step of a full round, and the partial sums' traffic.
-      const double step = esz == 4 ? (tile == 256 ? 7.2 : 3.7) : (tile == 256 ? 0.95 : 0.65);
+      const double step = esz == 4 ? 3.7 : tile == 256 ? 0.95 : 0.65;
       const double cost = rounds * (per * step + 3.0) + (splits > 1 ? 4.0 + 8.0 * splits * M * N / 4e6 : 0.0);
       if (cost < least) {
         least = cost;
@@ -550,8 +677,9 @@ void product(Product p, const Plan& plan, hipStream_t stream) {
   p.tiles_m = (int)((p.M + plan.tile - 1) / plan.tile);
   p.tiles_n = (int)((p.N + plan.tile - 1) / plan.tile);
   const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * plan.splits));
-  if (plan.tile == 256) hipLaunchKernelGGL((product_kernel<E, 256, 256, 2, 4, TA, TB>), grid, dim3(512), 0, stream, p);
-  else hipLaunchKernelGGL((product_kernel<E, 128, 128, 2, 2, TA, TB>), grid, dim3(256), 0, stream, p);
+  if constexpr (sizeof(E) == 2)
+    if (plan.tile == 256) hipLaunchKernelGGL((wide_product_kernel<E, TA, TB>), grid, dim3(256), 0, stream, p);
+  if (plan.tile == 128) hipLaunchKernelGGL((product_kernel<E, TA, TB>), grid, dim3(256), 0, stream, p);
   if (plan.splits > 1)
     hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)std::min<int64_t>((p.M * ((p.N * (int64_t)sizeof(E) + 15) / 16) + 255) / 256, kCus * 16)),
                        dim3(256), 0, stream, p.part, plan.splits, p.M, (int)p.N, p.epi);
