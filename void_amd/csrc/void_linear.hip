@@ -60,24 +60,23 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.442695040888963f));
 }
 
-// GELU in its tanh form: z sigmoid(2 u), u = 0.7978845608 (z + 0.044715 z^3).
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == VOID_ACT_RELU) return z < 0.f ? 0.f : z;
-  if (act == VOID_ACT_GELU) return z * sigmoid(1.5957691216f * z * fmaf(0.044715f * z, z, 1.f));
-  if (act == VOID_ACT_SILU) return z * sigmoid(z);
-  return z;
-}
-
-// Its derivative; beyond |z| = 30 it is 0 or 1 in fp32, and z^3 stays finite.
-__device__ __forceinline__ float slope_of(float z, int act) {
-  if (act == VOID_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  const float c = z > 30.f ? 30.f : z < -30.f ? -30.f : z;
-  if (act == VOID_ACT_GELU) {
-    const float s = sigmoid(1.5957691216f * c * fmaf(0.044715f * c, c, 1.f));
-    return fmaf(c * s * (1.f - s), 1.5957691216f * fmaf(0.134145f * c, c, 1.f), s);
+// z <- activation(z) and, where `want` is set, slope <- activation'(z).  GELU is
+// its tanh form z sigmoid(2 u), u = 0.7978845608 (z + 0.044715 z^3).  The slope's
+// z^2 is kept finite: it stands beside s (1 - s), which is 0 there.
+__device__ __forceinline__ void activate(float& z, float& slope, int act, bool want) {
+  if (act == VOID_ACT_RELU) {
+    slope = z > 0.f ? 1.f : 0.f;
+    z = z < 0.f ? 0.f : z;
+  } else if (act == VOID_ACT_GELU) {
+    const float s = sigmoid(1.5957691216f * z * fmaf(0.044715f * z, z, 1.f));
+    if (want)
+      slope = fmaf(z * (s * (1.f - s)), 1.5957691216f * fmaf(0.134145f, fminf(z * z, 1e4f), 1.f), s);
+    z *= s;
+  } else if (act == VOID_ACT_SILU) {
+    const float s = sigmoid(z);
+    if (want) slope = fmaf(z * s, 1.f - s, s);
+    z *= s;
   }
-  const float s = sigmoid(c);
-  return fmaf(c * s, 1.f - s, s);
 }
 
 struct Epilogue {
@@ -98,17 +97,18 @@ __device__ __forceinline__ float bias_at(const Epilogue& p, int64_t n) {
 
 template <class E>
 __device__ __forceinline__ void finish(const Epilogue& p, float sum, float bias, int64_t m, int64_t n, int64_t N) {
-  const float z = sum + bias;
-  if (p.slope) static_cast<typename Slope<E>::type*>(p.slope)[m * N + n] = Slope<E>::pack(slope_of(z, p.act));
-  float y = activate(z, p.act);
+  float y = sum + bias, slope = 0.f;
+  activate(y, slope, p.act, p.slope != nullptr);
+  if (p.slope) static_cast<typename Slope<E>::type*>(p.slope)[m * N + n] = Slope<E>::pack(slope);
   if (p.residual) y += (float)static_cast<const E*>(p.residual)[m * p.ldr + n];
   static_cast<E*>(p.out)[m * p.ldo + n] = (E)y;
 }
 
-// The same for a piece of n values of a row from column c on.
+// The same for a piece of n values of a row from column c on; `res` is the
+// residual's piece.
 template <class E>
 __device__ __forceinline__ void finish_piece(const Epilogue& p, typename Piece<E>::fvec z, const float (&bias)[Piece<E>::n],
-                                             int64_t m, int c, int N) {
+                                             typename Piece<E>::vec res, int64_t m, int c, int N) {
   constexpr int n = Piece<E>::n;
   typedef typename Piece<E>::fvec F;
   typedef typename Slope<E>::type S;
@@ -116,25 +116,41 @@ __device__ __forceinline__ void finish_piece(const Epilogue& p, typename Piece<E
   typedef SV SAny __attribute__((aligned(sizeof(S))));
 #pragma unroll
   for (int e = 0; e < n; ++e) z[e] += bias[e];
-  if (p.slope) {
-    S* sr = static_cast<S*>(p.slope) + m * N + c;
-    SV v;
+  if (p.act != VOID_ACT_NONE) {
+    F slope = 0.f;
+    auto all = [&](int act, bool want) {
 #pragma unroll
-    for (int e = 0; e < n; ++e) v[e] = Slope<E>::pack(slope_of(z[e], p.act));
-    if (c + n <= N) {
-      *reinterpret_cast<SAny*>(sr) = v;
-    } else {
+      for (int e = 0; e < n; ++e) {
+        float y = z[e], d = 0.f;
+        activate(y, d, act, want);
+        z[e] = y, slope[e] = d;
+      }
+    };
+    if (p.act == VOID_ACT_RELU) all(VOID_ACT_RELU, true);
+    else if (p.act == VOID_ACT_GELU) all(VOID_ACT_GELU, true);
+    else all(VOID_ACT_SILU, true);
+    if (p.slope) {
+      S* sr = static_cast<S*>(p.slope) + m * N + c;
+      SV v;
 #pragma unroll
-      for (int e = 0; e < n; ++e)
-        if (c + e < N) sr[e] = v[e];
+      for (int e = 0; e < n; ++e) v[e] = Slope<E>::pack(slope[e]);
+      if (c + n <= N) {
+        *reinterpret_cast<SAny*>(sr) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < n; ++e)
+          if (c + e < N) sr[e] = v[e];
+      }
     }
   }
-  if (p.act != VOID_ACT_NONE)
-#pragma unroll
-    for (int e = 0; e < n; ++e) z[e] = activate(z[e], p.act);
-  if (p.residual)
-    z += __builtin_convertvector(load_piece(static_cast<const E*>(p.residual) + m * p.ldr, c, N), F);
+  if (p.residual) z += __builtin_convertvector(res, F);
   store_piece(static_cast<E*>(p.out) + m * p.ldo, c, N, __builtin_convertvector(z, typename Piece<E>::vec));
+}
+
+template <class E>
+__device__ __forceinline__ typename Piece<E>::vec residual_piece(const Epilogue& p, int64_t m, int c, int N) {
+  if (!p.residual) return typename Piece<E>::vec{};
+  return load_piece(static_cast<const E*>(p.residual) + m * p.ldr, c, N);
 }
 
 template <class E>
@@ -208,14 +224,19 @@ struct Operand {
     }
   }
 
-  // Loads [F, T) of the next step into LDS, the last of them stepping on; `left`
-  // values of r remain from it on.
-  template <int F = 0, int T = kLoads>
+  // Load Q of the next step into LDS, the last of them stepping on; `left` values
+  // of r remain from it on.
+  template <int Q>
+  __device__ __forceinline__ void load_one(uint8_t* lds, int wave, int left) {
+    dma_b128(sgpr_rsrc(base), lds + (Q * NW + wave) * 1024, at[Q] < left ? voff[Q] : kOutOfRange, 0);
+    if (Q == kLoads - 1) base += step;
+  }
+  template <int... Q>
+  __device__ __forceinline__ void load_all(std::integer_sequence<int, Q...>, uint8_t* lds, int wave, int left) {
+    (load_one<Q>(lds, wave, left), ...);
+  }
   __device__ __forceinline__ void load(uint8_t* lds, int wave, int left) {
-    const v4s r = sgpr_rsrc(base);
-#pragma unroll
-    for (int q = F; q < T; ++q) dma_b128(r, lds + (q * NW + wave) * 1024, at[q] < left ? voff[q] : kOutOfRange, 0);
-    if (F < T && T == kLoads) base += step;
+    load_all(std::make_integer_sequence<int, kLoads>{}, lds, wave, left);
   }
 
   // Chunk pair kk's fragment of rows i0 .. i0 + 31: 16 bytes along r a lane.
@@ -270,27 +291,42 @@ struct Place {
   }
 };
 
-// 32 rows x COLS columns of sums from the wave's strip in LDS: whole pieces of
-// rows through the epilogue (or to the partial sums).
-template <class E, int COLS>
+// ROWS rows x COLS columns of sums from the wave's strip in LDS: whole pieces of
+// rows through the epilogue (or to the partial sums), four of them in flight.
+template <class E, int COLS, int ROWS>
 __device__ __forceinline__ void store_strip(const Product& p, int split, const float* strip, int64_t row0, int64_t col0,
                                             int lane) {
-  constexpr int kLanes = COLS / Piece<E>::n, kRows = 64 / kLanes;
-  const int c = lane % kLanes * Piece<E>::n, N = (int)p.N, col = (int)col0 + c;
-  float bias[Piece<E>::n];
+  constexpr int n = Piece<E>::n, kLanes = COLS / n, kRows = 64 / kLanes, kAhead = 4;
+  static_assert(ROWS % (kAhead * kRows) == 0);
+  typedef typename Piece<E>::fvec F;
+  const int c = lane % kLanes * n, N = (int)p.N, col = (int)col0 + c;
+  if (col >= N) return;
+  float bias[n];
   bias_piece<E>(p.epi, col, N, bias);
+  strip += lane / kLanes * COLS + c;
+  row0 += lane / kLanes;
 #pragma unroll 1
-  for (int q = lane / kLanes; q < 32; q += kRows) {
-    const int64_t row = row0 + q;
-    const typename Piece<E>::fvec z = *reinterpret_cast<const typename Piece<E>::fvec*>(strip + q * COLS + c);
-    if (row >= p.M || col >= N) continue;
-    if (p.part) {
-      float* d = p.part + ((int64_t)split * p.M + row) * N;
+  for (int q = 0; q < ROWS; q += kAhead * kRows) {
+    F z[kAhead];
+    typename Piece<E>::vec res[kAhead];
 #pragma unroll
-      for (int e = 0; e < Piece<E>::n; e += 4)
-        if (col + e < N) store_piece<float>(d, col + e, N, Piece<float>::vec{z[e], z[e + 1], z[e + 2], z[e + 3]});
-    } else {
-      finish_piece<E>(p.epi, z, bias, row, col, N);
+    for (int u = 0; u < kAhead; ++u) {
+      z[u] = *reinterpret_cast<const F*>(strip + (q + u * kRows) * COLS);
+      if (row0 + q + u * kRows < p.M) res[u] = residual_piece<E>(p.epi, row0 + q + u * kRows, col, N);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t row = row0 + q + u * kRows;
+      if (row >= p.M) continue;
+      if (p.part) {
+        float* d = p.part + ((int64_t)split * p.M + row) * N;
+#pragma unroll
+        for (int e = 0; e < n; e += 4)
+          if (col + e < N)
+            store_piece<float>(d, col + e, N, Piece<float>::vec{z[u][e], z[u][e + 1], z[u][e + 2], z[u][e + 3]});
+      } else {
+        finish_piece<E>(p.epi, z[u], bias, res[u], row, col, N);
+      }
     }
   }
 }
@@ -348,13 +384,21 @@ __global__ __launch_bounds__(256) void product_kernel(Product p) {
     }
   }
   __syncthreads();  // the last step is read
-  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * 64;
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 64 * 64;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < R; ++j) to_strip<64>(strip, 32 * j, acc[i][j], lane);
-    store_strip<E, 64>(p, at.split, strip, at.m0 + wm + 32 * i, at.n0 + wn, lane);
-  }
+    for (int j = 0; j < R; ++j) to_strip<64>(strip + i * 32 * 64, 32 * j, acc[i][j], lane);
+  store_strip<E, 64, 64>(p, at.split, strip, at.m0 + wm, at.n0 + wn, lane);
+}
+
+template <class F, int... Q>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, Q...>) {
+  (f(std::integral_constant<int, Q>{}), ...);
+}
+template <class F>
+__device__ __forceinline__ void each8(F f) {
+  each_of(f, std::make_integer_sequence<int, 8>{});
 }
 
 // 256 x 256 tiles of 16-bit operands, 4 waves of 128 x 128, one workgroup a CU: the
@@ -398,27 +442,24 @@ __global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
   // which the next set's products take them.
   auto phase = [&](auto kk_, const uint8_t* ra, const uint8_t* rb, auto load) {
     constexpr int kk = decltype(kk_)::value, next = (kk + 1) & 3, set = kk & 1, to = next & 1;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      if (q == 0) fb[to][0] = OpB::fragment(rb, wn, next, lane);
-      if (q == 1) fa[to][0] = OpA::fragment(ra, wm, next, lane);
-      if (q >= 2 && q <= 4) fb[to][q - 1] = OpB::fragment(rb, wn + 32 * (q - 1), next, lane);
-      if (q >= 5) fa[to][q - 4] = OpA::fragment(ra, wm + 32 * (q - 4), next, lane);
-      if (q == 0) load(std::integral_constant<int, 0>{});
-      if (q == 2) load(std::integral_constant<int, 1>{});
-      if (q == 4) load(std::integral_constant<int, 2>{});
-      if (q == 6) load(std::integral_constant<int, 3>{});
-      const int i = q >> 1, j = (q & 1) * 2;
+    auto two = [&](auto q_) {
+      constexpr int q = decltype(q_)::value, i = q >> 1, j = (q & 1) * 2;
+      if constexpr (q == 0) fb[to][0] = OpB::fragment(rb, wn, next, lane);
+      else if constexpr (q == 1) fa[to][0] = OpA::fragment(ra, wm, next, lane);
+      else if constexpr (q <= 4) fb[to][q - 1] = OpB::fragment(rb, wn + 32 * (q - 1), next, lane);
+      else fa[to][q - 4] = OpA::fragment(ra, wm + 32 * (q - 4), next, lane);
+      load(q_);
       acc[i][j] = mfma(fa[set][i], fb[set][j], acc[i][j], E{});
       acc[i][j + 1] = mfma(fa[set][i], fb[set][j + 1], acc[i][j + 1], E{});
       __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    each8(two);
   };
   a.load(const_cast<uint8_t*>(a0), wave, left(0));
   b.load(const_cast<uint8_t*>(b0), wave, left(0));
   a.load(const_cast<uint8_t*>(a1), wave, left(1));
-  b.template load<0, 4>(const_cast<uint8_t*>(b1), wave, left(1));
-  wait_vm<12>();
+  b.load(const_cast<uint8_t*>(b1), wave, left(1));
+  wait_vm<16>();
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -426,38 +467,36 @@ __global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
     fa[0][i] = OpA::fragment(a0, wm + 32 * i, 0, lane);
   }
   for (int s = 0; s < steps; ++s) {
-    const int l1 = left(s + 1), l2 = left(s + 2);
+    const int l2 = left(s + 2);
     phase(std::integral_constant<int, 0>{}, a0, b0, [&](auto q) {
-      constexpr int n = 4 + decltype(q)::value;
-      b.template load<n, n + 1>(const_cast<uint8_t*>(b1), wave, l1);
+      if constexpr (q.value % 2 == 0) a.template load_one<q.value / 2>(const_cast<uint8_t*>(a2), wave, l2);
     });
     phase(std::integral_constant<int, 1>{}, a0, b0, [&](auto q) {
-      constexpr int n = decltype(q)::value;
-      a.template load<n, n + 1>(const_cast<uint8_t*>(a2), wave, l2);
+      if constexpr (q.value % 2 == 0) a.template load_one<4 + q.value / 2>(const_cast<uint8_t*>(a2), wave, l2);
     });
-    phase(std::integral_constant<int, 2>{}, a0, b0, [&](auto q) {
-      constexpr int n = 4 + decltype(q)::value;
-      a.template load<n, n + 1>(const_cast<uint8_t*>(a2), wave, l2);
-    });
+    phase(std::integral_constant<int, 2>{}, a0, b0, [](auto) {});
     wait_vm<8>();     // A of step s + 2 stays in flight
     __syncthreads();  // step s is read, step s + 1 has landed
-    phase(std::integral_constant<int, 3>{}, a1, b1, [&](auto q) {
-      constexpr int n = decltype(q)::value;
-      b.template load<n, n + 1>(const_cast<uint8_t*>(b0), wave, l2);
-    });
+    phase(std::integral_constant<int, 3>{}, a1, b1,
+          [&](auto q) { b.template load_one<q.value>(const_cast<uint8_t*>(b0), wave, l2); });
     const uint8_t *a3 = a0, *b2 = b0;
     a0 = a1, a1 = a2, a2 = a3;
     b0 = b1, b1 = b2;
   }
   wait_vm<0>();     // loads past the last step still write zeros
   __syncthreads();
-  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * 128;
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 64 * 128;
+  each_of(
+      [&](auto h_) {
+        constexpr int h = 2 * decltype(h_)::value;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-#pragma unroll
-    for (int j = 0; j < R; ++j) to_strip<128>(strip, 32 * j, acc[i][j], lane);
-    store_strip<E, 128>(p, at.split, strip, at.m0 + wm + 32 * i, at.n0 + wn, lane);
-  }
+        for (int j = 0; j < R; ++j) {
+          to_strip<128>(strip, 32 * j, acc[h][j], lane);
+          to_strip<128>(strip + 32 * 128, 32 * j, acc[h + 1][j], lane);
+        }
+        store_strip<E, 128, 64>(p, at.split, strip, at.m0 + wm + 32 * h, at.n0 + wn, lane);
+      },
+      std::make_integer_sequence<int, 2>{});
 }
 
 // The splits' sums added in order, then the epilogue.
@@ -479,7 +518,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     }
     float bias[n];
     bias_piece<E>(epi, c, N, bias);
-    finish_piece<E>(epi, z, bias, m, c, N);
+    finish_piece<E>(epi, z, bias, residual_piece<E>(epi, m, c, N), m, c, N);
   }
 }
 
