@@ -188,12 +188,18 @@ __device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, _Float16) {
 //
 // Plain: row i at 128 i, its 16-byte chunks permuted by c ^ (i & 7), so that the
 // rows of a fragment read hit different banks.  Turned: row r of B values, its
-// chunks permuted by c ^ ((r & 3) << 2), for the transposing reads' 4 rows.  The
-// LDS-DMA writes lane after lane, so the permutation is in what each lane loads.
+// chunks permuted by c ^ swizzle(r), which keeps the 64 bytes that a transposing read
+// takes of each of 4 rows in different banks.  The LDS-DMA writes lane after lane, so
+// the permutation is in what each lane loads.
 template <class E, int B, int NW, bool TURNED>
 struct Operand {
   static constexpr int kPer = 16 / (int)sizeof(E), kBK = 128 / (int)sizeof(E), kLoads = B * 128 / (NW * 1024);
   static constexpr int kCpr = B * (int)sizeof(E) / 16;  // chunks of a turned row
+
+  // Of a turned row; only r & 3 counts.
+  static __device__ __forceinline__ constexpr int swizzle(int r) {
+    return kCpr >= 16 ? (r & 3) << 2 : kCpr == 8 ? (r & 2) << 1 : 0;
+  }
 
   const uint8_t* base;  // of the next step's first row / column
   int64_t step;         // bytes from step to step
@@ -217,7 +223,7 @@ struct Operand {
         voff[q] = i0 + row < I ? (int)(row * ld * (int64_t)sizeof(E)) + 16 * c : kOutOfRange;
         at[q] = c * kPer;
       } else {
-        const int row = id / kCpr, c = (id % kCpr) ^ ((row & 3) << 2);
+        const int row = id / kCpr, c = (id % kCpr) ^ swizzle(row);
         voff[q] = i0 + c * kPer < I ? (int)(row * ld * (int64_t)sizeof(E)) + 16 * c : kOutOfRange;
         at[q] = row;
       }
@@ -249,7 +255,7 @@ struct Operand {
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         f[s] = *reinterpret_cast<const float*>(lds + (8 * kk + 4 * g + s) * (B * 4) +
-                                               ((((i0 + j) >> 2) ^ (s << 2)) << 4) + (j & 3) * 4);
+                                               ((((i0 + j) >> 2) ^ swizzle(s)) << 4) + (j & 3) * 4);
       return __builtin_bit_cast(v4i, f);
     } else {
       // Two ds_read_b64_tr_b16: the 16 lanes of a read fetch 4 rows x 16 columns,
@@ -260,7 +266,7 @@ struct Operand {
       for (int r = 0; r < 2; ++r) {
         const int row = 16 * kk + 8 * g + 4 * r + (i >> 2);
         const int c = (i0 >> 3) + 2 * (j >> 4) + ((i & 3) >> 1);
-        const uint8_t* p = lds + row * (B * 2) + ((c ^ ((i >> 2) << 2)) << 4) + 8 * (i & 1);
+        const uint8_t* p = lds + row * (B * 2) + ((c ^ swizzle(i >> 2)) << 4) + 8 * (i & 1);
         t[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4h*)(const_cast<uint8_t*>(p)));
       }
       return __builtin_bit_cast(v4i, v8h{t[0][0], t[0][1], t[0][2], t[0][3], t[1][0], t[1][1], t[1][2], t[1][3]});
@@ -296,7 +302,7 @@ struct Place {
 template <class E, int COLS, int ROWS>
 __device__ __forceinline__ void store_strip(const Product& p, int split, const float* strip, int64_t row0, int64_t col0,
                                             int lane) {
-  constexpr int n = Piece<E>::n, kLanes = COLS / n, kRows = 64 / kLanes, kAhead = 4;
+  constexpr int n = Piece<E>::n, kLanes = COLS / n, kRows = 64 / kLanes, kAhead = ROWS / kRows < 4 ? ROWS / kRows : 4;
   static_assert(ROWS % (kAhead * kRows) == 0);
   typedef typename Piece<E>::fvec F;
   const int c = lane % kLanes * n, N = (int)p.N, col = (int)col0 + c;
@@ -339,57 +345,70 @@ __device__ __forceinline__ void to_strip(float* strip, int col, v16f acc, int la
   for (int r = 0; r < 16; ++r) strip[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * COLS + col + (lane & 31)] = acc[r];
 }
 
-// 128 x 128 tiles, 4 waves of 64 x 64, two steps in LDS, two workgroups a CU.
-template <class E, bool TA, bool TB>
-__global__ __launch_bounds__(256) void product_kernel(Product p) {
-  constexpr int B = 128, NW = 4, kBK = 128 / (int)sizeof(E), R = 2;
-  typedef Operand<E, B, NW, TA> OpA;
-  typedef Operand<E, B, NW, TB> OpB;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2 * B * 128];
+// BM x 128 tiles, 4 waves, two workgroups a CU.  BM = 128: waves of 64 x 64, two
+// steps in LDS.  BM = 64 and 32, for few rows: waves of BM x 32, three and four steps,
+// since there the operand that streams past is what bounds it, and bytes in flight
+// what that asks for.
+template <class E, int BM, bool TA, bool TB>
+__global__ __launch_bounds__(256, 2) void product_kernel(Product p) {
+  constexpr int BN = 128, NW = 4, kBK = 128 / (int)sizeof(E), kStages = BM == 128 ? 2 : BM == 64 ? 3 : 4;
+  constexpr int RA = BM == 128 ? 2 : BM / 32, RB = BM == 128 ? 2 : 1;
+  typedef Operand<E, BM, NW, TA> OpA;
+  typedef Operand<E, BN, NW, TB> OpB;
+  constexpr int kLoads = OpA::kLoads + OpB::kLoads;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages][(BM + BN) * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place<B, B> at(p, kBK);
+  const Place<BM, BN> at(p, kBK);
   const int steps = (int)((at.left + kBK - 1) / kBK);
   OpA a;
   OpB b;
   a.init(p.a, p.lda, at.m0, p.M, at.r0, wave, lane);
   b.init(p.b, p.ldb, at.n0, p.N, at.r0, wave, lane);
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  v16f acc[R][R];
+  const int wm = BM == 128 ? (wave >> 1) * 64 : 0, wn = BM == 128 ? (wave & 1) * 64 : wave * 32;
+  v16f acc[RA][RB];
 #pragma unroll
-  for (int i = 0; i < R; ++i)
+  for (int i = 0; i < RA; ++i)
 #pragma unroll
-    for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
-  auto load = [&](int s) {
-    const int l = (int)std::min<int64_t>(at.left - (int64_t)s * kBK, kBK);
-    a.load(&lds[s & 1][0], wave, l);
-    b.load(&lds[s & 1][B * 128], wave, l);
+    for (int j = 0; j < RB; ++j) acc[i][j] = 0.f;
+  // Past the last step nothing is left of r: such loads bring zeros and ask for no
+  // memory, and the waits can count.
+  auto load = [&](int s, int slot) {
+    const int l = (int)std::max<int64_t>(0, std::min<int64_t>(at.left - (int64_t)s * kBK, kBK));
+    a.load(&lds[slot][0], wave, l);
+    b.load(&lds[slot][BM * 128], wave, l);
   };
-  if (steps > 0) load(0);
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load(s, s);
+  int slot = 0, free = kStages - 1;
   for (int s = 0; s < steps; ++s) {
-    wait_vm<0>();
+    wait_vm<(kStages - 2) * kLoads>();
     __syncthreads();  // step s has landed everywhere, step s - 1 is read
-    if (s + 1 < steps) load(s + 1);
-    const uint8_t *la = &lds[s & 1][0], *lb = &lds[s & 1][B * 128];
+    load(s + kStages - 1, free);
+    const uint8_t *la = &lds[slot][0], *lb = &lds[slot][BM * 128];
+    free = slot;
+    slot = slot + 1 == kStages ? 0 : slot + 1;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      v4i fa[R], fb[R];
+      v4i fa[RA], fb[RB];
 #pragma unroll
-      for (int i = 0; i < R; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, kk, lane);
+      for (int i = 0; i < RA; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, kk, lane);
 #pragma unroll
-      for (int j = 0; j < R; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, kk, lane);
+      for (int j = 0; j < RB; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, kk, lane);
 #pragma unroll
-      for (int i = 0; i < R; ++i)
+      for (int i = 0; i < RA; ++i)
 #pragma unroll
-        for (int j = 0; j < R; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
+        for (int j = 0; j < RB; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
     }
   }
-  __syncthreads();  // the last step is read
-  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 64 * 64;
+  wait_vm<0>();     // loads past the last step still write zeros
+  __syncthreads();  // and the last step is read
+  constexpr int kRows = 32 * RA, kCols = 32 * RB;
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * kRows * kCols;
 #pragma unroll
-  for (int i = 0; i < R; ++i)
+  for (int i = 0; i < RA; ++i)
 #pragma unroll
-    for (int j = 0; j < R; ++j) to_strip<64>(strip + i * 32 * 64, 32 * j, acc[i][j], lane);
-  store_strip<E, 64, 64>(p, at.split, strip, at.m0 + wm, at.n0 + wn, lane);
+    for (int j = 0; j < RB; ++j) to_strip<kCols>(strip + i * 32 * kCols, 32 * j, acc[i][j], lane);
+  store_strip<E, kCols, kRows>(p, at.split, strip, at.m0 + wm, at.n0 + wn, lane);
 }
 
 template <class F, int... Q>
@@ -680,26 +699,32 @@ void by_type(int32_t dtype, Go go) {
   else go(_Float16{});
 }
 
-// A tile size and the K splits of a product.
+// Tile rows (the columns are 128, or 256 for 256) and the K splits of a product.
 struct Plan {
   int tile, splits, steps_per_split;
 };
 
+// The plan of least estimated time.  A CU takes one 256-row tile at a time or two of
+// the others; `step` is what a step of 128 bytes along r takes a full CU, in
+// microseconds as measured, `fixed` a tile's start and epilogue; splits add their
+// sums' traffic and a launch.
 Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
   const int64_t steps = std::max<int64_t>(1, (K * esz + 127) / 128);
   Plan best{128, 1, (int)steps};
   double least = 1e300;
-  for (int tile : {256, 128}) {
+  for (int tile : {256, 128, 64, 32}) {
     if (tile == 256 && esz == 4) continue;
-    const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+    const int64_t width = tile == 256 ? 256 : 128;
+    const int64_t tiles = ((M + tile - 1) / tile) * ((N + width - 1) / width);
     const int64_t slots = kCus * (tile == 256 ? 1 : 2);
-    for (int splits = 1; splits <= 16 && splits <= steps; ++splits) {
+    const double step = esz == 4 ? (tile == 128 ? 3.7 : tile == 64 ? 1.9 : 1.0)
+                                 : (tile == 256 ? 1.5 : tile == 128 ? 1.1 : tile == 64 ? 0.8 : 0.65);
+    const double fixed = tile == 256 ? 15.0 : tile == 128 ? 8.0 : 5.0;
+    for (int splits = 1; splits <= 32 && splits <= steps; ++splits) {
       const int64_t per = (steps + splits - 1) / splits;
       if (splits > 1 && ((steps + per - 1) / per != splits || per < 4)) continue;
       const int64_t rounds = (tiles * splits + slots - 1) / slots;
-      // Microseconds: a step of a full round, and the partial sums' traffic.
-      const double step = esz == 4 ? 3.7 : tile == 256 ? 0.95 : 0.65;
-      const double cost = rounds * (per * step + 3.0) + (splits > 1 ? 4.0 + 8.0 * splits * M * N / 4e6 : 0.0);
+      const double cost = rounds * (per * step + fixed) + (splits > 1 ? 4.0 + 8.0 * splits * M * N / 4e6 : 0.0);
       if (cost < least) {
         least = cost;
         best = Plan{tile, splits, (int)per};
@@ -714,11 +739,13 @@ void product(Product p, const Plan& plan, hipStream_t stream) {
   p.splits = plan.splits;
   p.steps_per_split = plan.steps_per_split;
   p.tiles_m = (int)((p.M + plan.tile - 1) / plan.tile);
-  p.tiles_n = (int)((p.N + plan.tile - 1) / plan.tile);
+  p.tiles_n = (int)((p.N + (plan.tile == 256 ? 255 : 127)) / (plan.tile == 256 ? 256 : 128));
   const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * plan.splits));
   if constexpr (sizeof(E) == 2)
     if (plan.tile == 256) hipLaunchKernelGGL((wide_product_kernel<E, TA, TB>), grid, dim3(256), 0, stream, p);
-  if (plan.tile == 128) hipLaunchKernelGGL((product_kernel<E, TA, TB>), grid, dim3(256), 0, stream, p);
+  if (plan.tile == 128) hipLaunchKernelGGL((product_kernel<E, 128, TA, TB>), grid, dim3(256), 0, stream, p);
+  if (plan.tile == 64) hipLaunchKernelGGL((product_kernel<E, 64, TA, TB>), grid, dim3(256), 0, stream, p);
+  if (plan.tile == 32) hipLaunchKernelGGL((product_kernel<E, 32, TA, TB>), grid, dim3(256), 0, stream, p);
   if (plan.splits > 1)
     hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)std::min<int64_t>((p.M * ((p.N * (int64_t)sizeof(E) + 15) / 16) + 255) / 256, kCus * 16)),
                        dim3(256), 0, stream, p.part, plan.splits, p.M, (int)p.N, p.epi);
@@ -741,7 +768,10 @@ void few(const void_linear_args* d, const Epilogue& epi, hipStream_t stream) {
   else waves(std::integral_constant<int, 4>{});
 }
 
+// Up to 64 tokens take operands of any alignment; more than 16 go through the tiles
+// where the operands allow it (the waves of few_kernel would read X again and again).
 bool few_tokens(int64_t M) { return M <= 64; }
+bool few_by_rows(int64_t M, bool whole) { return M <= 16 || (M <= 64 && !whole); }
 
 // Rows that the LDS-DMA reads in whole chunks: aligned, of whole chunks.
 bool whole_chunks(const void* p, int64_t ld, int64_t cols, int esz) {
@@ -766,7 +796,7 @@ extern "C" {
 int32_t void_linear_any_alignment(int64_t M) { return few_tokens(M); }
 
 size_t void_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-  if (M <= 0 || N <= 0 || few_tokens(M)) return 0;
+  if (M <= 0 || N <= 0 || few_by_rows(M, true)) return 0;
   const Plan p = plan_of(M, N, K, size_of(dtype));
   return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
 }
@@ -789,11 +819,12 @@ int void_linear(const void_linear_args* d, hipStream_t stream) {
       (d->bias && (uintptr_t)d->bias % size_of(d->bias_dtype)))
     return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
   const Epilogue epi{d->y, d->ldy, d->bias, d->residual, d->ldr, d->slope, d->bias_dtype == VOID_DT_F32, d->activation};
-  if (few_tokens(d->M)) {
+  const bool whole = d->K == 0 || (whole_chunks(d->x, d->ldx, d->K, esz) && whole_chunks(d->w, d->ldw, d->K, esz));
+  if (few_by_rows(d->M, whole)) {
     by_type(d->dtype, [&](auto e) { few<decltype(e)>(d, epi, stream); });
     return launched();
   }
-  if (d->K && (!whole_chunks(d->x, d->ldx, d->K, esz) || !whole_chunks(d->w, d->ldw, d->K, esz)))
+  if (!whole)
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "more than 64 tokens need rows of whole 16-byte chunks");
   if (256 * std::max(d->ldx, d->ldw) * esz > INT_MAX - 65536)
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
