@@ -704,33 +704,48 @@ struct Plan {
   int tile, splits, steps_per_split;
 };
 
-// The plan of least estimated time.  A CU takes one 256-row tile at a time or two of
-// the others; `step` is what a step of 128 bytes along r takes a full CU, in
-// microseconds as measured, `fixed` a tile's start and epilogue; splits add their
-// sums' traffic and a launch.
+// The plan of least estimated time, in microseconds.  A CU takes one 256-row tile at
+// a time, or two of the others: `fixed` is a tile's start and epilogue, `alone` and
+// `full` a step of 128 bytes along r where a CU has one tile and, per tile, where it
+// has two; splits add a launch and their sums' traffic.  The figures are fitted to 400
+// timings of 18 bf16 and 8 fp32 products (17 to 8192 rows, 512 to 14336 columns, depths
+// of 512 to 14336; the estimates are within 15 %, the plans chosen 2 % and 0.4 % slower
+// than each product's best).
+struct Cost {
+  int tile;
+  double fixed, alone, full, join, traffic;
+};
+
+constexpr Cost kCost16[] = {{256, 11.7, 1.17, 1.17, 3.0, 1.2},
+                            {128, 3.7, 0.77, 0.55, 3.2, 1.0},
+                            {64, 0.8, 0.45, 0.39, 4.9, 1.3},
+                            {32, 1.9, 0.35, 0.29, 5.0, 0.85}};
+constexpr Cost kCost32[] = {{128, 1.3, 2.07, 1.96, 4.8, 1.0}, {64, 1.0, 1.12, 1.03, 4.5, 1.15}, {32, 2.7, 0.65, 0.57, 3.0, 1.0}};
+
 Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
   const int64_t steps = std::max<int64_t>(1, (K * esz + 127) / 128);
-  Plan best{128, 1, (int)steps};
+  Plan best{};
   double least = 1e300;
-  for (int tile : {256, 128, 64, 32}) {
-    if (tile == 256 && esz == 4) continue;
-    const int64_t width = tile == 256 ? 256 : 128;
-    const int64_t tiles = ((M + tile - 1) / tile) * ((N + width - 1) / width);
-    const int64_t slots = kCus * (tile == 256 ? 1 : 2);
-    const double step = esz == 4 ? (tile == 128 ? 3.7 : tile == 64 ? 1.9 : 1.0)
-                                 : (tile == 256 ? 1.5 : tile == 128 ? 1.1 : tile == 64 ? 0.8 : 0.65);
-    const double fixed = tile == 256 ? 15.0 : tile == 128 ? 8.0 : 5.0;
+  auto consider = [&](const Cost& c) {
+    const int64_t width = c.tile == 256 ? 256 : 128;
+    const int64_t tiles = ((M + c.tile - 1) / c.tile) * ((N + width - 1) / width);
     for (int splits = 1; splits <= 32 && splits <= steps; ++splits) {
       const int64_t per = (steps + splits - 1) / splits;
       if (splits > 1 && ((steps + per - 1) / per != splits || per < 4)) continue;
-      const int64_t rounds = (tiles * splits + slots - 1) / slots;
-      const double cost = rounds * (per * step + fixed) + (splits > 1 ? 4.0 + 8.0 * splits * M * N / 4e6 : 0.0);
+      const int64_t each = (tiles * splits + kCus - 1) / kCus;  // tiles of the fullest CU
+      const double one = c.fixed + per * c.alone, two = c.fixed + per * std::max(c.alone, 2 * c.full);
+      double cost = c.tile == 256 ? each * one : each / 2 * two + each % 2 * (one - 0.3 * c.fixed);
+      if (splits > 1) cost += c.join + c.traffic * splits * M * N / 1e6;
       if (cost < least) {
         least = cost;
-        best = Plan{tile, splits, (int)per};
+        best = Plan{c.tile, splits, (int)per};
       }
     }
-  }
+  };
+  if (esz == 4)
+    for (const Cost& c : kCost32) consider(c);
+  else
+    for (const Cost& c : kCost16) consider(c);
   return best;
 }
 
@@ -768,10 +783,15 @@ void few(const void_linear_args* d, const Epilogue& epi, hipStream_t stream) {
   else waves(std::integral_constant<int, 4>{});
 }
 
-// Up to 64 tokens take operands of any alignment; more than 16 go through the tiles
-// where the operands allow it (the waves of few_kernel would read X again and again).
+// Up to 64 tokens take operands of any alignment, through few_kernel.  Where the
+// operands allow the tiles, more than 16 tokens take them (few_kernel's waves read X
+// again and again: 32 tokens x 14336 x 4096 bf16 52 us, tiles 29), and two to 16 where
+// the weight is larger than 64 MiB (16 tokens of the same 36.7 us, tiles 27.6; x 4096 x
+// 4096 12.9, and 16.9 with the tiles' second launch).
 bool few_tokens(int64_t M) { return M <= 64; }
-bool few_by_rows(int64_t M, bool whole) { return M <= 16 || (M <= 64 && !whole); }
+bool few_by_rows(int64_t M, int64_t N, int64_t K, int esz, bool whole) {
+  return M == 1 || (M <= 16 && N * K * esz <= (int64_t)64 << 20) || (M <= 64 && !whole);
+}
 
 // Rows that the LDS-DMA reads in whole chunks: aligned, of whole chunks.
 bool whole_chunks(const void* p, int64_t ld, int64_t cols, int esz) {
@@ -796,7 +816,7 @@ extern "C" {
 int32_t void_linear_any_alignment(int64_t M) { return few_tokens(M); }
 
 size_t void_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-  if (M <= 0 || N <= 0 || few_by_rows(M, true)) return 0;
+  if (M <= 0 || N <= 0 || few_by_rows(M, N, K, size_of(dtype), true)) return 0;
   const Plan p = plan_of(M, N, K, size_of(dtype));
   return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
 }
@@ -820,7 +840,7 @@ int void_linear(const void_linear_args* d, hipStream_t stream) {
     return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
   const Epilogue epi{d->y, d->ldy, d->bias, d->residual, d->ldr, d->slope, d->bias_dtype == VOID_DT_F32, d->activation};
   const bool whole = d->K == 0 || (whole_chunks(d->x, d->ldx, d->K, esz) && whole_chunks(d->w, d->ldw, d->K, esz));
-  if (few_by_rows(d->M, whole)) {
+  if (few_by_rows(d->M, d->N, d->K, esz, whole)) {
     by_type(d->dtype, [&](auto e) { few<decltype(e)>(d, epi, stream); });
     return launched();
   }
