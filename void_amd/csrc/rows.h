@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 namespace {
 
@@ -68,6 +70,12 @@ __device__ __forceinline__ void load_params(float (&f)[N], const W* p, int c, in
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = c + e < cols ? (float)p[c + e] : 0.f;
   }
+}
+
+// f(0), f(1), ..., as integral constants: an unrolled loop whose indexes stay constants.
+template <class F, int... Q>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, Q...>) {
+  (f(std::integral_constant<int, Q>{}), ...);
 }
 
 // Sum over the aligned group of T lanes (a power of two up to 64) that holds this lane.

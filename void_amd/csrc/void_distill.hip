@@ -55,50 +55,77 @@ struct Args {
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- reductions over the T threads of a workgroup -------------------------
+//
+// One barrier each: every kind has an area of its own in LDS, and an area is
+// written again only behind another barrier that follows its reads.
+
+struct Areas {
+  float max[16], sum[16];
+  int flags[16];
+};
 
 template <int T>
-__device__ __forceinline__ float max_over(float v, float* red) {
+__device__ __forceinline__ float max_over(float v, Areas& r) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
   if constexpr (T > 64) {
-    __syncthreads();  // red is free
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) r.max[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[0];
+    v = r.max[0];
 #pragma unroll
-    for (int w = 1; w < T / 64; ++w) v = fmaxf(v, red[w]);
+    for (int w = 1; w < T / 64; ++w) v = fmaxf(v, r.max[w]);
   }
   return v;
 }
 
 template <int T>
-__device__ __forceinline__ float sum_over(float v, float* red) {
+__device__ __forceinline__ float sum_over(float v, Areas& r) {
   v = lanes_sum<64>(v);
   if constexpr (T > 64) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) r.sum[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0.f;
 #pragma unroll
-    for (int w = 0; w < T / 64; ++w) v += red[w];
+    for (int w = 0; w < T / 64; ++w) v += r.sum[w];
   }
   return v;
+}
+
+// The two low bits of v, or-ed: put() before a barrier, get() behind it.
+template <int T>
+__device__ __forceinline__ int put_flags(int v, Areas& r) {
+  const int f = (__ballot(v & 1) ? 1 : 0) | (__ballot(v & 2) ? 2 : 0);
+  if (T > 64 && (threadIdx.x & 63) == 0) r.flags[threadIdx.x >> 6] = f;
+  return f;
+}
+template <int T>
+__device__ __forceinline__ int get_flags(int f, const Areas& r) {
+  if constexpr (T > 64) {
+    f = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) f |= r.flags[w];
+  }
+  return __builtin_amdgcn_readfirstlane(f);
 }
 
 // ---- the teacher's entries of a row ---------------------------------------
 
+constexpr int kSome = 1, kBad = 2;  // the row has an entry; one is past the vocabulary
+
 // In dynamic LDS, k of each.
 struct Entries {
-  float* p;     // probability; 0 where the entry does not count
-  float* lp;    // its logarithm
   int32_t* at;  // index, -1 where the entry does not count
+  float* t;     // the teacher's logit, later its probability
+  float* s;     // the student's logit there
 };
 
+constexpr int pad4(int k) { return (k + 3) & ~3; }
+
 __device__ __forceinline__ Entries entries_of(float* lds, int k) {
-  return Entries{lds, lds + k, reinterpret_cast<int32_t*>(lds + 2 * k)};
+  return Entries{reinterpret_cast<int32_t*>(lds), lds + pad4(k), lds + 2 * pad4(k)};
 }
 
-size_t entries_bytes(int k) { return (size_t)std::max(k, 1) * 12; }
+size_t entries_bytes(int k) { return (size_t)pad4(std::max(k, 1)) * 12; }
 
 __device__ __forceinline__ int64_t entry_index(const Args& a, int64_t row, int j) {
   return a.index_bytes == 8 ? static_cast<const int64_t*>(a.index)[row * a.ldi + j]
@@ -114,66 +141,137 @@ __device__ __forceinline__ float entry_logit(const Args& a, int64_t row, int j) 
 
 __device__ __forceinline__ bool entry_counts(int64_t at, float t) { return at >= 0 && !(t == -INFINITY); }
 
-// Whether the row has an entry that counts (the same for all T threads).
+// A row's entries on their way to LDS, entry threadIdx.x + i T in place i.
 template <int T>
-__device__ __forceinline__ bool has_entries(const Args& a, int64_t row) {
-  int any = 0;
-  for (int j = threadIdx.x; j < a.k; j += T) any |= entry_counts(entry_index(a, row, j), entry_logit(a, row, j));
-  if constexpr (T == 64) return __ballot(any) != 0;
-  else return __syncthreads_or(any) != 0;
-}
+struct Raw {
+  static constexpr int kPer = kMaxEntries / T;
+  int32_t at[kPer];
+  float t[kPer];
+  int flags;  // of this thread's entries
 
-// The row's entries into `en`; false (and nothing usable in en) where none
-// counts.  Ends behind a barrier.
-template <int T>
-__device__ __forceinline__ bool load_entries(const Args& a, int64_t row, const Entries& en, float* red) {
-  __syncthreads();  // en is free
-  float top = -INFINITY;
-  int bad = 0;
-  for (int j = threadIdx.x; j < a.k; j += T) {
-    const int64_t at = entry_index(a, row, j);
-    const float t = entry_logit(a, row, j);
-    const bool use = entry_counts(at, t);
-    bad |= use && at >= a.vocab;
-    en.at[j] = use ? (int32_t)(at < a.vocab ? at : 0) : -1;
-    en.lp[j] = t;
-    if (use) top = fmaxf(top, t == t ? t : kLowest);  // a NaN still counts
+  __device__ __forceinline__ void fetch(const Args& a, int64_t row) {
+    flags = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = i * T + (int)threadIdx.x;
+      if (i * T < a.k && j < a.k) {
+        const int64_t v = entry_index(a, row, j);
+        t[i] = entry_logit(a, row, j);
+        const bool use = entry_counts(v, t[i]);
+        at[i] = !use ? -1 : v < a.vocab ? (int32_t)v : 0;
+        flags |= !use ? 0 : v < a.vocab ? kSome : kSome | kBad;
+      }
+    }
   }
-  top = max_over<T>(top, red);
-  if (top == -INFINITY) return false;
-  float s = bad ? NAN : 0.f;
-  for (int j = threadIdx.x; j < a.k; j += T) {
-    const float d = (en.lp[j] - top) * a.c, e = en.at[j] >= 0 ? pow2(d) : 0.f;
-    en.p[j] = e;
-    en.lp[j] = d;
-    s += e;
+  __device__ __forceinline__ void put(const Args& a, const Entries& en) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = i * T + (int)threadIdx.x;
+      if (i * T < a.k && j < a.k) {
+        en.at[j] = at[i];
+        en.t[j] = t[i];
+      }
+    }
+    // Up to a multiple of 4, for reads of 4 at a time.
+    if ((int)threadIdx.x < pad4(a.k) - a.k) en.at[a.k + threadIdx.x] = -1;
   }
-  s = sum_over<T>(s, red);
-  const float inv = 1.f / s, ls = logf(s);
-  for (int j = threadIdx.x; j < a.k; j += T) {
-    en.p[j] *= inv;
-    en.lp[j] = en.lp[j] * 0.693147180559945309f - ls;
-  }
-  __syncthreads();
-  return true;
-}
+};
 
-// The row's loss from its entries and its m and z.
+// The student's logits at a row's entries, for the thread's own.
 template <class E, int T>
-__device__ __forceinline__ float row_loss(const Args& a, const E* s, const Entries& en, float m, float z, float* red) {
-  const float lz = logf(z), t = a.temperature;
-  float sum = 0.f;
-  for (int j = threadIdx.x; j < a.k; j += T) {
-    const float p = en.p[j];
-    if (en.at[j] >= 0 && p != 0.f) sum += p * (en.lp[j] + (lz - ((float)s[en.at[j]] - m) / t));
+struct Gathered {
+  static constexpr int kPer = kMaxEntries / T;
+  float s[kPer];
+  __device__ __forceinline__ void fetch(const Args& a, const E* row, const Entries& en) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = i * T + (int)threadIdx.x;
+      if (i * T < a.k && j < a.k) s[i] = (float)row[max(en.at[j], 0)];
+    }
   }
-  return sum_over<T>(sum, red) * t * t;
+  __device__ __forceinline__ void put(const Args& a, const Entries& en) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = i * T + (int)threadIdx.x;
+      if (i * T < a.k && j < a.k) en.s[j] = s[i];
+    }
+  }
+};
+
+// All that a row's entries ask for, by one wave (the others go on): p, the loss
+// (returned) from m and z = sum exp2((s - m) c), and, unless ds is null, the
+// gradients of the entries' logits with index in [lo, hi), where the first of equal
+// indices writes, with all their p.  Everything else of the gradient is written.
+template <class E>
+__device__ __forceinline__ float entries_by_wave(const Args& a, const Entries& en, int flags, float m, float z, float gs,
+                                                 int64_t lo, int64_t hi, E* ds) {
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY;
+  for (int j = lane; j < a.k; j += 64)
+    if (en.at[j] >= 0) {
+      const float t = en.t[j];
+      top = fmaxf(top, t == t ? t : kLowest);  // a NaN still counts
+    }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  float sum = 0.f;
+  for (int j = lane; j < a.k; j += 64)
+    if (en.at[j] >= 0) sum += pow2((en.t[j] - top) * a.c);
+  sum = flags & kBad ? NAN : lanes_sum<64>(sum);
+  const float inv = 1.f / sum, back = logf(z) - logf(sum);
+  float loss = 0.f;
+  for (int j = lane; j < a.k; j += 64) {
+    const float d = en.t[j] - top, p = en.at[j] >= 0 ? pow2(d * a.c) * inv : 0.f;
+    // log p - log q = (t - top) / T - log sum - (s - m) / T + log z
+    if (p != 0.f) loss += p * ((d - (en.s[j] - m)) / a.temperature + back);
+    en.t[j] = p;
+  }
+  loss = lanes_sum<64>(loss) * a.temperature * a.temperature;
+  if (ds) {
+    const float iz = 1.f / z;
+    for (int j = lane; j < a.k; j += 64) {
+      const int at = en.at[j];
+      if (at < lo || at >= hi) continue;
+      float p = 0.f;
+      bool first = true;
+      for (int i = 0; i < a.k; i += 4) {
+        const int4 q = *reinterpret_cast<const int4*>(en.at + i);
+        if (q.x == at || q.y == at || q.z == at || q.w == at) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w) == at) {
+              first &= i + e >= j;
+              p += en.t[i + e];
+            }
+        }
+      }
+      if (first) ds[at] = (E)(gs * (pow2((en.s[j] - m) * a.c) * iz - p));
+    }
+  }
+  return loss;
 }
 
-// ---- sums over the vocabulary ----------------------------------------------
+// ---- slices of a row ---------------------------------------------------------
 
 struct Part {  // largest logit and sum exp2((s - m) c) of a row or of a slice
   float m, z;
+};
+
+// Slice s of S: whole pieces [first, last), and, the last slice, the row's `rest`
+// values behind them.
+template <class E>
+struct Slice {
+  static constexpr int N = Piece<E>::n;
+  uint32_t first, last, rest;
+  int64_t lo, hi;  // its columns
+  __device__ __forceinline__ Slice(int vocab, int S, int s) {
+    const uint32_t whole = (uint32_t)vocab / N, per = (whole + S - 1) / S;
+    first = min(per * s, whole);
+    last = min(first + per, whole);
+    rest = s == S - 1 ? (uint32_t)vocab % N : 0;
+    lo = (int64_t)first * N;
+    hi = (int64_t)last * N + rest;
+  }
 };
 
 __device__ __forceinline__ Part join(Part x, Part y, float c) {
@@ -181,35 +279,31 @@ __device__ __forceinline__ Part join(Part x, Part y, float c) {
   return Part{m, x.z * pow2((x.m - m) * c) + y.z * pow2((y.m - m) * c)};
 }
 
-// (m, z) of pieces [first, last) of a row, for all T threads.  Each thread
-// keeps its own largest logit and rescales its sum when a batch of kAhead
-// pieces raises it.
+// (m, z) of a slice, for all T threads.  Each thread keeps its own largest logit and
+// rescales its sum when a batch of kAhead pieces raises it.
 template <class E, int T>
-__device__ __forceinline__ Part row_part(const Args& a, const E* s, int first, int last, float* red) {
+__device__ __forceinline__ Part slice_part(const Args& a, const E* s, const Slice<E>& sl, Areas& red) {
   constexpr int N = Piece<E>::n, kAhead = 4;
+  typedef typename Piece<E>::any Any;
   typedef typename Piece<E>::fvec F;
   float m = kLowest, z = 0.f;
-  for (int64_t q = first + threadIdx.x; q < last; q += kAhead * T) {
+  if (threadIdx.x < sl.rest) {
+    const float x = (float)s[(int64_t)sl.last * N + threadIdx.x];
+    m = fmaxf(m, x);
+    z = pow2((x - m) * a.c);
+  }
+  for (uint32_t q = sl.first + threadIdx.x; q < sl.last; q += kAhead * T) {
     typename Piece<E>::vec v[kAhead];
-    bool whole[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int64_t c0 = (q + u * T) * N;
-      whole[u] = q + u * T < last && c0 + N <= a.vocab;
-      if (whole[u]) v[u] = *reinterpret_cast<const typename Piece<E>::any*>(s + c0);
+      v[u] = (E)-INFINITY;
+      if (q + u * T < sl.last) v[u] = *reinterpret_cast<const Any*>(s + (int64_t)(q + u * T) * N);
     }
-    F f[kAhead];
     float top = m;
+    F f[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (whole[u]) f[u] = __builtin_convertvector(v[u], F);
-      else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int64_t c = (q + u * T) * N + e;
-          f[u][e] = q + u * T < last && c < a.vocab ? (float)s[c] : -INFINITY;
-        }
-      }
+      f[u] = __builtin_convertvector(v[u], F);
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, f[u][e]);
     }
@@ -239,37 +333,31 @@ __device__ __forceinline__ Part join_parts(const float2* parts, int S, float c) 
   return Part{__shfl(p.m, 0, 64), __shfl(p.z, 0, 64)};
 }
 
-// Pieces [first, last) of slice s of S.
-__device__ __forceinline__ void slice(int pieces, int S, int s, int& first, int& last) {
-  const int per = (pieces + S - 1) / S;
-  first = (int)std::min<int64_t>((int64_t)s * per, pieces);
-  last = std::min(first + per, pieces);
+template <class E, int T>
+__device__ __forceinline__ void zero_slice(E* ds, const Slice<E>& sl) {
+  typedef typename Piece<E>::any Any;
+  for (uint32_t q = sl.first + threadIdx.x; q < sl.last; q += T)
+    *reinterpret_cast<Any*>(ds + (int64_t)q * Piece<E>::n) = typename Piece<E>::vec{};
+  if (threadIdx.x < sl.rest) ds[(int64_t)sl.last * Piece<E>::n + threadIdx.x] = (E)0.f;
 }
 
-// ---- gradient --------------------------------------------------------------
-
-// The gradient of the entries' logits with index in [lo, hi): the first of
-// equal indices writes, with all their p.
+// A row's entries into LDS, with its logits there where it has any; its flags.  Ends
+// behind a barrier that the entries are behind too (the logits only where `wait`).
 template <class E, int T>
-__device__ __forceinline__ void entry_grads(const Args& a, const E* s, const Entries& en, Part st, float gs, int64_t lo,
-                                            int64_t hi, E* ds) {
-  for (int j = threadIdx.x; j < a.k; j += T) {
-    const int at = en.at[j];
-    if (at < lo || at >= hi) continue;
-    float p = 0.f;
-    bool first = true;
-    for (int i = 0; i < a.k; ++i)
-      if (en.at[i] == at) {
-        first &= i >= j;
-        p += en.p[i];
-      }
-    if (first) ds[at] = (E)(gs * (pow2(((float)s[at] - st.m) * a.c) / st.z - p));
+__device__ __forceinline__ int take_entries(const Args& a, int64_t row, const E* s, const Entries& en, Areas& red) {
+  Raw<T> raw;
+  raw.fetch(a, row);
+  __syncthreads();  // en is free
+  raw.put(a, en);
+  int flags = put_flags<T>(raw.flags, red);
+  __syncthreads();
+  flags = get_flags<T>(flags, red);
+  if (flags & kSome) {
+    Gathered<E, T> g;
+    g.fetch(a, s, en);
+    g.put(a, en);
   }
-}
-
-template <class E, int T>
-__device__ __forceinline__ void zero_pieces(E* ds, int vocab, int first, int last) {
-  for (int q = first + threadIdx.x; q < last; q += T) store_piece<E>(ds, q * Piece<E>::n, vocab, {});
+  return flags;
 }
 
 // ---- kernels ---------------------------------------------------------------
@@ -279,55 +367,65 @@ __device__ __forceinline__ void zero_pieces(E* ds, int vocab, int first, int las
 template <class E, int T, bool LOSS>
 __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t units, float2* __restrict__ parts,
                                                           int32_t* __restrict__ used, float* __restrict__ loss) {
-  __shared__ float red[16];
-  extern __shared__ float lds[];
+  __shared__ Areas red;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const Entries en = entries_of(lds, a.k);
-  const int pieces = (int)(((int64_t)a.vocab + Piece<E>::n - 1) / Piece<E>::n);
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t row = u / S;
     const int sl = (int)(u - row * S);
     const E* s = static_cast<const E*>(a.logits) + row * a.ld;
-    const bool some = LOSS ? load_entries<T>(a, row, en, red) : has_entries<T>(a, row);
+    int flags;
+    if constexpr (LOSS) {
+      flags = take_entries<E, T>(a, row, s, en, red);
+    } else {
+      Raw<T> raw;
+      raw.fetch(a, row);
+      flags = put_flags<T>(raw.flags, red);
+      __syncthreads();
+      flags = get_flags<T>(flags, red);
+    }
     Part p{0.f, 1.f};
-    float l = 0.f;
-    if (some) {
-      int first, last;
-      slice(pieces, S, sl, first, last);
-      p = row_part<E, T>(a, s, first, last, red);
-      if constexpr (LOSS) l = row_loss<E, T>(a, s, en, p.m, p.z, red);
+    if (flags & kSome) p = slice_part<E, T>(a, s, Slice<E>(a.vocab, S, sl), red);
+    if (threadIdx.x < 64) {
+      float l = 0.f;
+      if (LOSS && flags & kSome) l = entries_by_wave<E>(a, en, flags, p.m, p.z, 0.f, 0, 0, nullptr);
+      if (threadIdx.x == 0) {
+        parts[u] = make_float2(p.m, p.z);
+        if (sl == 0) used[row] = flags & kSome;
+        if constexpr (LOSS) loss[row] = l;
+      }
     }
-    if (threadIdx.x == 0) {
-      parts[u] = make_float2(p.m, p.z);
-      if (sl == 0) used[row] = some;
-      if constexpr (LOSS) loss[row] = l;
-    }
+    if constexpr (!LOSS) __syncthreads();  // the areas are free
   }
 }
 
-// The losses of rows whose parts were made in slices.
+// The losses of rows whose parts were made in slices; a wave a row.
 template <class E>
-__global__ __launch_bounds__(256) void distill_loss_kernel(Args a, int S, const float2* __restrict__ parts,
-                                                           float* __restrict__ loss) {
-  __shared__ float red[16];
-  extern __shared__ float lds[];
+__global__ __launch_bounds__(64) void distill_loss_kernel(Args a, int S, const float2* __restrict__ parts,
+                                                          float* __restrict__ loss) {
+  __shared__ Areas red;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const Entries en = entries_of(lds, a.k);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float l = 0.f;
-    if (load_entries<256>(a, row, en, red)) {
+    const int flags = take_entries<E, 64>(a, row, static_cast<const E*>(a.logits) + row * a.ld, en, red);
+    if (flags & kSome) {
       const Part p = join_parts(parts + row * S, S, a.c);
-      l = row_loss<E, 256>(a, static_cast<const E*>(a.logits) + row * a.ld, en, p.m, p.z, red);
+      l = entries_by_wave<E>(a, en, flags, p.m, p.z, 0.f, 0, 0, nullptr);
     }
     if (threadIdx.x == 0) loss[row] = l;
   }
 }
 
-// n counts of rows with entries, for all T threads.
+// n counts of rows with entries, for all T threads.  Ends behind a barrier.
 template <int T>
-__device__ __forceinline__ float total_count(const int32_t* counts, int n, float* red) {
-  // Exact in fp32 sums of parts below 2^24 each; a mean over more rows rounds.
+__device__ __forceinline__ float total_count(const int32_t* counts, int n, Areas& red) {
+  // Exact while a thread's part stays below 2^24; a mean over more rows rounds.
   int64_t c = 0;
   for (int i = threadIdx.x; i < n; i += T) c += counts[i];
-  return sum_over<T>((float)c, red);
+  const float s = sum_over<T>((float)c, red);
+  __syncthreads();
+  return s;
 }
 
 // Gradient, unit u = (row, slice) of G.  The upstream gradient is g[row * gstep],
@@ -342,49 +440,51 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
                                                          E* __restrict__ grad, int64_t ldg, float* __restrict__ loss) {
   constexpr int N = Piece<E>::n, kAhead = 4;
   typedef typename Piece<E>::vec V;
+  typedef typename Piece<E>::any Any;
   typedef typename Piece<E>::fvec F;
-  __shared__ float red[16];
-  extern __shared__ float lds[];
+  __shared__ Areas red;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const Entries en = entries_of(lds, a.k);
-  const int pieces = (int)(((int64_t)a.vocab + N - 1) / N);
   if (factor) scale *= *factor;
   if (counts) scale /= fmaxf(total_count<T>(counts, n_counts, red), 1.f);
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t row = u / G;
-    const int sl = (int)(u - row * G);
+    const int n = (int)(u - row * G);
+    const Slice<E> sl(a.vocab, G, n);
     const E* s = static_cast<const E*>(a.logits) + row * a.ld;
     E* ds = grad + row * ldg;
-    int first, last;
-    slice(pieces, G, sl, first, last);
-    if (!load_entries<T>(a, row, en, red)) {
-      zero_pieces<E, T>(ds, a.vocab, first, last);
-      if (loss && sl == 0 && threadIdx.x == 0) loss[row] = 0.f;
+    const int flags = take_entries<E, T>(a, row, s, en, red);
+    if (!(flags & kSome)) {
+      zero_slice<E, T>(ds, sl);
+      if (loss && n == 0 && threadIdx.x == 0) loss[row] = 0.f;
       continue;
     }
     const Part st = join_parts(parts + row * S, S, a.c);
-    if (loss && sl == 0) {
-      const float l = row_loss<E, T>(a, s, en, st.m, st.z, red);
-      if (threadIdx.x == 0) loss[row] = l;
-    }
     const float gs = (g ? g[row * gstep] * scale : scale) * a.temperature;
-    // A row made NaN by an index past the vocabulary shows it everywhere.
-    const float f = en.p[0] == en.p[0] ? gs / st.z : NAN;
-    for (int64_t q = first + threadIdx.x; q < last; q += kAhead * T) {
+    const float f = flags & kBad ? NAN : gs / st.z;
+    for (uint32_t q = sl.first + threadIdx.x; q < sl.last; q += kAhead * T) {
       V v[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
-        if (q + i * T < last) v[i] = load_piece(s, (int)((q + i * T) * N), a.vocab);
+        if (q + i * T < sl.last) v[i] = *reinterpret_cast<const Any*>(s + (int64_t)(q + i * T) * N);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
-        if (q + i * T < last) {
+        if (q + i * T < sl.last) {
           F o = __builtin_convertvector(v[i], F);
 #pragma unroll
           for (int e = 0; e < N; ++e) o[e] = pow2((o[e] - st.m) * a.c) * f;
-          store_piece(ds, (int)((q + i * T) * N), a.vocab, __builtin_convertvector(o, V));
+          *reinterpret_cast<Any*>(ds + (int64_t)(q + i * T) * N) = __builtin_convertvector(o, V);
         }
     }
+    if (threadIdx.x < sl.rest) {
+      const int64_t c = (int64_t)sl.last * N + threadIdx.x;
+      ds[c] = (E)(pow2(((float)s[c] - st.m) * a.c) * f);
+    }
     __syncthreads();  // the entries' logits are written again
-    entry_grads<E, T>(a, s, en, st, gs, (int64_t)first * N, (int64_t)last * N, ds);
+    if (threadIdx.x < 64) {
+      const float l = entries_by_wave<E>(a, en, flags, st.m, st.z, gs, sl.lo, sl.hi, ds);
+      if (loss && n == 0 && threadIdx.x == 0) loss[row] = l;
+    }
   }
 }
 
@@ -412,78 +512,127 @@ __global__ __launch_bounds__(1024) void distill_count_kernel(Args a, int32_t* __
 }
 
 // Loss and gradient of whole rows, NV pieces a thread in registers between the
-// two.
+// two.  As a row's pieces are written the next row's are loaded in their place, so
+// that memory works on while the sums are made; the next row's entries are fetched
+// before this row's sums, and one wave does this row's while the others go on.
 template <class E, int T, int NV>
-__global__ __launch_bounds__(T) void distill_step_kernel(Args a, float scale, const int32_t* __restrict__ counts,
-                                                         int n_counts, E* __restrict__ grad, int64_t ldg,
-                                                         float* __restrict__ loss, int32_t* __restrict__ used) {
+__global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale, const int32_t* __restrict__ counts,
+                                                            int n_counts, E* __restrict__ grad, int64_t ldg,
+                                                            float* __restrict__ loss, int32_t* __restrict__ used) {
   constexpr int N = Piece<E>::n;
   typedef typename Piece<E>::vec V;
+  typedef typename Piece<E>::any Any;
   typedef typename Piece<E>::fvec F;
-  __shared__ float red[16];
-  extern __shared__ float lds[];
-  const Entries en = entries_of(lds, a.k);
+  __shared__ Areas red;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   if (counts) scale /= fmaxf(total_count<T>(counts, n_counts, red), 1.f);
-  const int pieces = (int)(((int64_t)a.vocab + N - 1) / N);
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const E* s = static_cast<const E*>(a.logits) + row * a.ld;
+  const float gs = scale * a.temperature;
+  V v[NV];
+  // Whole pieces in v; the row's last vocab % N values one a thread in `last`.
+  E last = (E)-INFINITY;
+  const uint32_t whole = (uint32_t)a.vocab / N, rest = (uint32_t)a.vocab % N;
+  const std::make_integer_sequence<int, NV> pieces_each;
+  // The compiler is kept from holding the pieces' offsets through the loop over the
+  // rows, and every value widened from one loop over the pieces to the next.
+  auto fresh = [](uint32_t t) {
+    asm volatile("" : "+v"(t));
+    return t;
+  };
+  auto forget = [&] {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
+  };
+  auto fetch = [&](const E* s, auto i_) {
+    constexpr int i = decltype(i_)::value;
+    const uint32_t q = (uint32_t)i * T + fresh(threadIdx.x);
+    v[i] = (E)-INFINITY;
+    if (q < whole) v[i] = *reinterpret_cast<const Any*>(s + q * N);
+    if (i == 0 && threadIdx.x < rest) last = s[whole * N + threadIdx.x];
+  };
+  auto row_at = [&](int64_t r) { return static_cast<const E*>(a.logits) + r * a.ld; };
+  auto entries_at = [&](int turn) { return entries_of(lds + turn * 3 * pad4(a.k), a.k); };
+  int64_t row = blockIdx.x;
+  Raw<T> raw;
+  raw.fetch(a, row);
+  raw.put(a, entries_at(0));
+  int flags = put_flags<T>(raw.flags, red);
+  __syncthreads();
+  flags = get_flags<T>(flags, red);
+  if (flags & kSome) each_of([&](auto i) { fetch(row_at(row), i); }, pieces_each);
+  for (int turn = 0; row < a.rows; turn ^= 1) {
+    const int64_t next = row + gridDim.x;
+    const Entries en = entries_at(turn);
+    const E *s = row_at(row), *sn = row_at(next);
     E* ds = grad + row * ldg;
-    const bool some = load_entries<T>(a, row, en, red);
-    if (threadIdx.x == 0) used[row] = some;
-    if (!some) {
-      zero_pieces<E, T>(ds, a.vocab, 0, pieces);
-      if (threadIdx.x == 0) loss[row] = 0.f;
-      continue;
+    const bool some = flags & kSome;
+    raw.flags = 0;
+    if (next < a.rows) raw.fetch(a, next);
+    float m = kLowest, z = 0.f;
+    const float tail = (float)last;
+    if (some) {
+      Gathered<E, T> at;
+      at.fetch(a, s, en);
+      each_of(
+          [&](auto i) {
+            const F f = __builtin_convertvector(v[i.value], F);
+#pragma unroll
+            for (int e = 0; e < N; ++e) m = fmaxf(m, f[e]);
+            __builtin_amdgcn_sched_barrier(0);
+          },
+          pieces_each);
+      m = max_over<T>(fmaxf(m, tail), red);
+      at.put(a, en);
+      forget();
+      each_of(
+          [&](auto i) {
+            const F f = __builtin_convertvector(v[i.value], F);
+#pragma unroll
+            for (int e = 0; e < N; ++e) z += pow2((f[e] - m) * a.c);
+            __builtin_amdgcn_sched_barrier(0);
+          },
+          pieces_each);
+      z += pow2((tail - m) * a.c);
+      forget();
+    } else {
+      __syncthreads();  // the other entries, read by the first wave, are free
     }
-    V v[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * T + (int)threadIdx.x) * N;
-      if (c + N <= a.vocab) v[i] = *reinterpret_cast<const typename Piece<E>::any*>(s + c);
-      else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i][e] = c + e < a.vocab ? s[c + e] : (E)-INFINITY;
-      }
-    }
-    // Without these the compiler keeps every value widened from one loop to the
-    // next, at twice the registers.
-    auto forget = [&] {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
-    };
-    float m = kLowest;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const F f = __builtin_convertvector(v[i], F);
-#pragma unroll
-      for (int e = 0; e < N; ++e) m = fmaxf(m, f[e]);
-    }
-    m = max_over<T>(m, red);
-    forget();
-    float z = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const F f = __builtin_convertvector(v[i], F);
-#pragma unroll
-      for (int e = 0; e < N; ++e) z += pow2((f[e] - m) * a.c);
-    }
+    // Behind the barrier of the maximum, or this one, the first wave is done with the
+    // row before, whose entries the next row's replace.
+    if (next < a.rows) raw.put(a, entries_at(turn ^ 1));
+    int more = put_flags<T>(raw.flags, red);
     z = sum_over<T>(z, red);
-    forget();
-    const float gs = scale * a.temperature, f0 = en.p[0] == en.p[0] ? gs / z : NAN;
+    more = get_flags<T>(more, red);
+    if (some) {
+      const float f0 = flags & kBad ? NAN : gs / z;
+      each_of(
+          [&](auto i_) {
+            constexpr int i = decltype(i_)::value;
+            const uint32_t q = (uint32_t)i * T + fresh(threadIdx.x);
+            if (q < whole) {
+              F o = __builtin_convertvector(v[i], F);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * T + (int)threadIdx.x) * N;
-      if (c < a.vocab) {
-        F o = __builtin_convertvector(v[i], F);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = pow2((o[e] - m) * a.c) * f0;
-        store_piece(ds, c, a.vocab, __builtin_convertvector(o, V));
+              for (int e = 0; e < N; ++e) o[e] = pow2((o[e] - m) * a.c) * f0;
+              *reinterpret_cast<Any*>(ds + q * N) = __builtin_convertvector(o, V);
+            }
+            if (i == 0 && threadIdx.x < rest) ds[whole * N + threadIdx.x] = (E)(pow2((tail - m) * a.c) * f0);
+            if (more & kSome) fetch(sn, i_);
+            __builtin_amdgcn_sched_barrier(0);
+          },
+          pieces_each);
+      __syncthreads();  // the entries' logits are written again
+      if (threadIdx.x < 64) {
+        const float l = entries_by_wave<E>(a, en, flags, m, z, gs, 0, a.vocab, ds);
+        if (threadIdx.x == 0) loss[row] = l;
       }
+    } else {
+      zero_slice<E, T>(ds, Slice<E>(a.vocab, 1, 0));
+      if (threadIdx.x == 0) loss[row] = 0.f;
+      if (more & kSome) each_of([&](auto i) { fetch(sn, i); }, pieces_each);
+      __syncthreads();  // the flags are read
     }
-    const float l = row_loss<E, T>(a, s, en, m, z, red);
-    if (threadIdx.x == 0) loss[row] = l;
-    __syncthreads();
-    entry_grads<E, T>(a, s, en, Part{m, z}, gs, 0, a.vocab, ds);
+    if (threadIdx.x == 0) used[row] = some;
+    row = next;
+    flags = more;
   }
 }
 
@@ -492,7 +641,7 @@ __global__ __launch_bounds__(T) void distill_step_kernel(Args a, float scale, co
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ loss,
                                                            const int32_t* __restrict__ used, int64_t rows, int mean,
                                                            float* __restrict__ out, float* __restrict__ factor) {
-  __shared__ float red[16];
+  __shared__ Areas red;
   float s = 0.f;
   int64_t n = 0;
   for (int64_t r = threadIdx.x; r < rows; r += 1024) {
@@ -500,6 +649,7 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
     n += used[r];
   }
   s = sum_over<1024>(s, red);
+  __syncthreads();
   const float c = sum_over<1024>((float)n, red);
   const float f = mean ? 1.f / fmaxf(c, 1.f) : 1.f;
   if (threadIdx.x == 0) {
@@ -582,7 +732,7 @@ void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, hipSt
       hipLaunchKernelGGL((distill_parts_kernel<E, T, false>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss);
   });
   if (S > 1 && loss)
-    hipLaunchKernelGGL(distill_loss_kernel<E>, dim3((unsigned)std::min(a.rows, kMaxGrid)), dim3(256), entries_bytes(a.k), stream, a, S,
+    hipLaunchKernelGGL(distill_loss_kernel<E>, dim3((unsigned)std::min(a.rows, kMaxGrid)), dim3(64), entries_bytes(a.k), stream, a, S,
                        part, loss);
 }
 
@@ -609,7 +759,7 @@ bool by_row(int vocab, Go go) {
   VOID_ROW(256, 2);
   VOID_ROW(256, 4);
   VOID_ROW(256, 8);
-  VOID_ROW(256, 16);
+  VOID_ROW(512, 8);
   VOID_ROW(1024, 8);
   VOID_ROW(1024, 16);
 #undef VOID_ROW
@@ -697,7 +847,8 @@ int void_distill_step(const void_distill_args* d, int32_t mean, float grad_scale
             constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
             count();
             hipLaunchKernelGGL((distill_step_kernel<E, T, NV>),
-                               dim3((unsigned)std::min<int64_t>(d->rows, kCus * (2048 / T))), dim3(T), entries_bytes(a.k), stream, a,
+                               dim3((unsigned)std::min<int64_t>(d->rows, kCus * (1024 / T))), dim3(T),
+                               2 * entries_bytes(a.k), stream, a,
                                grad_scale, mean ? counts : nullptr, n, static_cast<E*>(grad), ldg, row_loss, used);
           }))
         return;

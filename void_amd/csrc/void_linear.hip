@@ -411,10 +411,6 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Product p) {
   store_strip<E, kCols, kRows>(p, at.split, strip, at.m0 + wm, at.n0 + wn, lane);
 }
 
-template <class F, int... Q>
-__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, Q...>) {
-  (f(std::integral_constant<int, Q>{}), ...);
-}
 template <class F>
 __device__ __forceinline__ void each8(F f) {
   each_of(f, std::make_integer_sequence<int, 8>{});
