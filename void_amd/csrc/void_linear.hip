@@ -38,15 +38,15 @@ typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 // act'(Z), kept for the backward pass: fp32 for fp32 values, else 16-bit fixed
 // point 2^15 s + 2^13 (s lies in [-0.13, 1.13] for every activation; 0 and 1 are
 // exact, others within 2^-16: a tenth of a bf16 rounding of dZ, where a slope
-// rounded to bf16 would add another whole one).  65535 stands for NaN.
+// rounded to bf16 would add another whole one).  NaN becomes 0, which no slope takes.
 template <class E>
 struct Slope {
   typedef uint16_t type;
   static __device__ __forceinline__ uint16_t pack(float s) {
-    return s == s ? (uint16_t)(int)rintf(fmaf(s, 32768.f, 8192.f)) : (uint16_t)65535;
+    return (uint16_t)__float2uint_rz(fmaf(s, 32768.f, 8192.5f));
   }
   static __device__ __forceinline__ float unpack(uint16_t u) {
-    return u == 65535 ? __builtin_nanf("") : ((float)u - 8192.f) * (1.f / 32768.f);
+    return u ? fmaf((float)u, 1.f / 32768.f, -0.25f) : __builtin_nanf("");
   }
 };
 template <>
@@ -68,10 +68,12 @@ __device__ __forceinline__ void activate(float& z, float& slope, int act, bool w
     slope = z > 0.f ? 1.f : 0.f;
     z = z < 0.f ? 0.f : z;
   } else if (act == VOID_ACT_GELU) {
-    const float s = sigmoid(1.5957691216f * z * fmaf(0.044715f * z, z, 1.f));
-    if (want)
-      slope = fmaf(z * (s * (1.f - s)), 1.5957691216f * fmaf(0.134145f, fminf(z * z, 1e4f), 1.f), s);
-    z *= s;
+    // sigmoid(2 u) = 1 / (1 + 2^-(2 log2(e) u)); 2 du/dz = 1.5957691 + 0.2140644 z^2.
+    const float z2 = z * z;
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * fmaf(z2, -0.10294324f, -2.30220819f)));
+    const float y = z * s;
+    if (want) slope = fmaf(y * (1.f - s), fmaf(fminf(z2, 1e4f), 0.21406442f, 1.5957691216f), s);
+    z = y;
   } else if (act == VOID_ACT_SILU) {
     const float s = sigmoid(z);
     if (want) slope = fmaf(z * s, 1.f - s, s);
@@ -184,6 +186,13 @@ __device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, _Float16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0, 0, 0);
+}
+
 // One operand's B rows (of the tile) x 128 bytes along r, in LDS.
 //
 // Plain: row i at 128 i, its 16-byte chunks permuted by c ^ (i & 7), so that the
@@ -243,6 +252,14 @@ struct Operand {
   }
   __device__ __forceinline__ void load(uint8_t* lds, int wave, int left) {
     load_all(std::make_integer_sequence<int, kLoads>{}, lds, wave, left);
+  }
+
+  // Half kk (32 of r) of a plain operand's rows i0 .. i0 + 15 for the 16 x 16 x 32
+  // instructions: lane (i, g) holds r = 8 g .. 8 g + 7 of row i.  16-bit values.
+  static __device__ __forceinline__ v4i fragment16(const uint8_t* lds, int i0, int kk, int lane) {
+    static_assert(!TURNED && sizeof(E) == 2);
+    const int i = lane & 15, g = lane >> 4;
+    return *reinterpret_cast<const v4i*>(lds + (i0 + i) * 128 + (((4 * kk + g) ^ (i & 7)) << 4));
   }
 
   // Chunk pair kk's fragment of rows i0 .. i0 + 31: 16 bytes along r a lane.
@@ -514,6 +531,96 @@ __global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
       std::make_integer_sequence<int, 2>{});
 }
 
+// The same for two plain operands on the 16 x 16 x 32 instructions, whose sums cost
+// the matrix cores less energy (they take half as many steps along r); the chip runs
+// these tiles at its power limit: 8192 x 14336 x 4096 bf16 739 us against 773.  A step
+// is two fragment sets.
+template <class E>
+__global__ __launch_bounds__(256, 1) void wide_plain_kernel(Product p) {
+  constexpr int B = 256, NW = 4, kBK = 64, R = 8, kOperand = B * 128;
+  typedef Operand<E, B, NW, false> OpA;
+  typedef OpA OpB;
+  static_assert(OpA::kLoads == 8 && OpB::kLoads == 8);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[5][kOperand];  // A: 0 1 2, B: 3 4
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place<B, B> at(p, kBK);
+  const int steps = (int)((at.left + kBK - 1) / kBK);
+  OpA a;
+  OpB b;
+  a.init(p.a, p.lda, at.m0, p.M, at.r0, wave, lane);
+  b.init(p.b, p.ldb, at.n0, p.N, at.r0, wave, lane);
+  const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
+  v4f acc[R][R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+  // What is left of r at step s; past the last step nothing: such loads bring zeros
+  // and ask for no memory.
+  auto left = [&](int s) { return (int)std::max<int64_t>(0, std::min<int64_t>(at.left - (int64_t)s * kBK, kBK)); };
+  v4i fa[2][R], fb[2][R];
+  // Where A of this step, the next and the one after next are, and B of this and the next.
+  const uint8_t *a0 = lds[0], *a1 = lds[1], *a2 = lds[2], *b0 = lds[3], *b1 = lds[4];
+  // Set kk's products, four at a time behind one of the other set's sixteen reads and,
+  // every second time, one of the phase's eight loads.  The reads come in the order in
+  // which the next products take them.
+  auto phase = [&](auto kk_, const uint8_t* ra, const uint8_t* rb, auto load) {
+    constexpr int set = decltype(kk_)::value, to = set ^ 1;
+    auto four = [&](auto q_) {
+      constexpr int q = decltype(q_)::value, i = q >> 1, j = (q & 1) * 4;
+      if constexpr (q == 0) fb[to][0] = OpB::fragment16(rb, wn, to, lane);
+      else if constexpr (q == 1) fa[to][0] = OpA::fragment16(ra, wm, to, lane);
+      else if constexpr (q <= 8) fb[to][q - 1] = OpB::fragment16(rb, wn + 16 * (q - 1), to, lane);
+      else fa[to][q - 8] = OpA::fragment16(ra, wm + 16 * (q - 8), to, lane);
+      if constexpr (q % 2 == 0) load(std::integral_constant<int, q / 2>{});
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc[i][j + u] = mfma16(fa[set][i], fb[set][j + u], acc[i][j + u], E{});
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each_of(four, std::make_integer_sequence<int, 16>{});
+  };
+  a.load(const_cast<uint8_t*>(a0), wave, left(0));
+  b.load(const_cast<uint8_t*>(b0), wave, left(0));
+  a.load(const_cast<uint8_t*>(a1), wave, left(1));
+  b.load(const_cast<uint8_t*>(b1), wave, left(1));
+  wait_vm<16>();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    fb[0][i] = OpB::fragment16(b0, wn + 16 * i, 0, lane);
+    fa[0][i] = OpA::fragment16(a0, wm + 16 * i, 0, lane);
+  }
+  for (int s = 0; s < steps; ++s) {
+    const int l2 = left(s + 2);
+    phase(std::integral_constant<int, 0>{}, a0, b0,
+          [&](auto q) { a.template load_one<q.value>(const_cast<uint8_t*>(a2), wave, l2); });
+    wait_vm<8>();     // A of step s + 2 stays in flight
+    __syncthreads();  // step s is read, step s + 1 has landed
+    phase(std::integral_constant<int, 1>{}, a1, b1,
+          [&](auto q) { b.template load_one<q.value>(const_cast<uint8_t*>(b0), wave, l2); });
+    const uint8_t *a3 = a0, *b2 = b0;
+    a0 = a1, a1 = a2, a2 = a3;
+    b0 = b1, b1 = b2;
+  }
+  wait_vm<0>();     // loads past the last step still write zeros
+  __syncthreads();
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 64 * 128;
+  each_of(
+      [&](auto h_) {
+        constexpr int h = 4 * decltype(h_)::value;
+        // Lane (j, g) holds column j and rows 4 g .. 4 g + 3 of each 16 x 16.
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              strip[(16 * i + 4 * (lane >> 4) + r) * 128 + 16 * j + (lane & 15)] = acc[h + i][j][r];
+        store_strip<E, 128, 64>(p, at.split, strip, at.m0 + wm + 16 * h, at.n0 + wn, lane);
+      },
+      std::make_integer_sequence<int, 2>{});
+}
+
 // The splits' sums added in order, then the epilogue.
 template <class E>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t M, int N,
@@ -753,7 +860,10 @@ void product(Product p, const Plan& plan, hipStream_t stream) {
   p.tiles_n = (int)((p.N + (plan.tile == 256 ? 255 : 127)) / (plan.tile == 256 ? 256 : 128));
   const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * plan.splits));
   if constexpr (sizeof(E) == 2)
-    if (plan.tile == 256) hipLaunchKernelGGL((wide_product_kernel<E, TA, TB>), grid, dim3(256), 0, stream, p);
+    if (plan.tile == 256) {
+      if constexpr (!TA && !TB) hipLaunchKernelGGL(wide_plain_kernel<E>, grid, dim3(256), 0, stream, p);
+      else hipLaunchKernelGGL((wide_product_kernel<E, TA, TB>), grid, dim3(256), 0, stream, p);
+    }
   if (plan.tile == 128) hipLaunchKernelGGL((product_kernel<E, 128, TA, TB>), grid, dim3(256), 0, stream, p);
   if (plan.tile == 64) hipLaunchKernelGGL((product_kernel<E, 64, TA, TB>), grid, dim3(256), 0, stream, p);
   if (plan.tile == 32) hipLaunchKernelGGL((product_kernel<E, 32, TA, TB>), grid, dim3(256), 0, stream, p);
