@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define VOID_AMD_ABI_VERSION 5
+#define VOID_AMD_ABI_VERSION 6
 #define VOID_TILE 32
 
 typedef enum void_status {

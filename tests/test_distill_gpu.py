@@ -277,6 +277,19 @@ def test_streams_and_graphs(gpu):
         assert torch.equal(void_amd.distillation_loss_and_grad(s, t, idx)[1], want[1])
 
 
+@gpu_only
+def test_forward_mode_and_second_derivatives_are_refused(gpu):
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.randn(4, 16, device=gpu), torch.ones(4, 16, device=gpu))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            void_amd.distillation_loss(x, torch.zeros(4, 2, device=gpu), torch.zeros(4, 2, dtype=torch.int64, device=gpu))
+    x = torch.randn(4, 16, device=gpu, requires_grad=True)
+    g, = torch.autograd.grad(void_amd.distillation_loss(x, torch.zeros(4, 2, device=gpu), torch.zeros(4, 2, dtype=torch.int64, device=gpu)).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_refusals():
     s, t, i = torch.randn(2, 50), torch.randn(2, 4), torch.zeros(2, 4, dtype=torch.int64)
     for call in (void_amd.distillation_loss, void_amd.distillation_loss_and_grad):

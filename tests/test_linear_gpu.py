@@ -289,6 +289,19 @@ def test_graph_replays(gpu, M, K):
         assert torch.equal(void_amd.fused_linear(x, w, b, "gelu", r), want)
 
 
+@gpu_only
+def test_forward_mode_and_second_derivatives_are_refused(gpu):
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.randn(4, 16, device=gpu), torch.ones(4, 16, device=gpu))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            void_amd.fused_linear(x, torch.randn(8, 16, device=gpu))
+    x = torch.randn(4, 16, device=gpu, requires_grad=True)
+    g, = torch.autograd.grad(void_amd.fused_linear(x, torch.randn(8, 16, device=gpu)).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_refusals():
     x, w = torch.randn(2, 8), torch.randn(4, 8)
     f = void_amd.fused_linear

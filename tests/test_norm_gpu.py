@@ -221,6 +221,19 @@ def test_graph_replays(gpu):
         assert torch.equal(void_amd.layer_norm(x, w, b), want)
 
 
+@gpu_only
+def test_forward_mode_and_second_derivatives_are_refused(gpu):
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.randn(4, 16, device=gpu), torch.ones(4, 16, device=gpu))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            void_amd.layer_norm(x)
+    x = torch.randn(4, 16, device=gpu, requires_grad=True)
+    g, = torch.autograd.grad(void_amd.layer_norm(x).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_refusals():
     x = torch.randn(2, 8)
     with pytest.raises(RuntimeError, match="GPU"):

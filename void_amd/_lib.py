@@ -12,7 +12,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libvoid_amd.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # Scratch limits of void_spmm_int8_noalloc (VOID_NOALLOC_*_BYTES)
 NOALLOC_COUNTER_BYTES = 1 << 20

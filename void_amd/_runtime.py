@@ -18,6 +18,7 @@ from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, tuning
 from ._streams import raw_stream, record_once
@@ -66,6 +67,14 @@ def float_code(t: torch.Tensor, what: str) -> int:
     if code is None:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
+
+
+def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on these tensors is recorded by autograd.  Within a
+    forward-mode level always, where autograd raises for tangents that an
+    operator does not take."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled()
+                                              and any(t is not None and t.requires_grad for t in tensors))
 
 
 def flat_rows(t: torch.Tensor) -> torch.Tensor:

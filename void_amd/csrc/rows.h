@@ -125,4 +125,30 @@ struct RowSum {
   }
 };
 
+// Column c of n rows of `pitch` floats, added in order by a workgroup of 1024: each
+// wave every 16th row, eight of them in flight, then the waves in order.  The result
+// is the first wave's (0 past the last column).
+__device__ __forceinline__ float partial_rows_sum(const float* part, int n, int64_t pitch, int64_t c,
+                                                  float (&sum)[16][64]) {
+  constexpr int kAhead = 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float a[kAhead] = {};
+  if (c < pitch) {
+    int k = wave;
+    for (; k + 16 * (kAhead - 1) < n; k += 16 * kAhead)
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) a[u] += part[(k + 16 * u) * pitch + c];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (k + 16 * u < n) a[u] += part[(k + 16 * u) * pitch + c];
+  }
+  sum[wave][lane] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+  __syncthreads();
+  float s = 0.f;
+  if (wave == 0)
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += sum[w][lane];
+  return s;
+}
+
 }  // namespace

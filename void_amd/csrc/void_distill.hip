@@ -608,9 +608,21 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
   __shared__ Areas red;
   float s = 0.f;
   int64_t n = 0;
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-    s += loss[r];
-    n += used[r];
+  // Four rows in flight; a thread's are added in order.
+  for (int64_t r = threadIdx.x; r < rows; r += 4 * 1024) {
+    float l[4];
+    int u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = r + i * 1024 < rows;
+      l[i] = in ? loss[r + i * 1024] : 0.f;
+      u[i] = in ? used[r + i * 1024] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s += l[i];
+      n += u[i];
+    }
   }
   s = sum_over<1024>(s, red);
   __syncthreads();

@@ -173,12 +173,6 @@ struct Product {
   Epilogue epi;
 };
 
-__device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, float) {
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(v4f, a)[s], __builtin_bit_cast(v4f, b)[s], c, 0, 0, 0);
-  return c;
-}
 __device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c, __bf16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
@@ -411,10 +405,19 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Product p) {
       for (int i = 0; i < RA; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, kk, lane);
 #pragma unroll
       for (int j = 0; j < RB; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, kk, lane);
+      // fp32: one of the chunk's four values at a time, so that products in a row are
+      // of different sums.
 #pragma unroll
-      for (int i = 0; i < RA; ++i)
+      for (int u = 0; u < (sizeof(E) == 4 ? 4 : 1); ++u)
 #pragma unroll
-        for (int j = 0; j < RB; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
+        for (int i = 0; i < RA; ++i)
+#pragma unroll
+          for (int j = 0; j < RB; ++j)
+            if constexpr (sizeof(E) == 4)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(v4f, fa[i])[u],
+                                                               __builtin_bit_cast(v4f, fb[j])[u], acc[i][j], 0, 0, 0);
+            else
+              acc[i][j] = mfma(fa[i], fb[j], acc[i][j], E{});
     }
   }
   wait_vm<0>();     // loads past the last step still write zeros
@@ -770,17 +773,13 @@ __global__ __launch_bounds__(256) void slope_kernel(const E* __restrict__ dy, in
   }
 }
 
+// db: the n partial rows added in order, 16 at a time (one a wave), and rounded once.
 template <class W>
-__global__ __launch_bounds__(256) void bias_sum_kernel(const float* __restrict__ part, int n, int N, W* __restrict__ db) {
-  __shared__ float sum[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.f;
-  if (c < N)
-    for (int k = wave; k < n; k += 4) s += part[(int64_t)k * N + c];
-  sum[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && c < N) db[c] = (W)((sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]));
+__global__ __launch_bounds__(1024) void bias_sum_kernel(const float* __restrict__ part, int n, int N, W* __restrict__ db) {
+  __shared__ float sum[16][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = partial_rows_sum(part, n, N, c, sum);
+  if (threadIdx.x < 64 && c < N) db[c] = (W)s;
 }
 
 // ---- host ---------------------------------------------------------------------
@@ -1067,10 +1066,10 @@ int void_linear_grad_z(const void* dy, int64_t lddy, const void* slope, int64_t 
     if (db) {
       const dim3 grid((unsigned)((N + 63) / 64));
       if (bias_dtype == VOID_DT_F32)
-        hipLaunchKernelGGL(bias_sum_kernel<float>, grid, dim3(256), 0, stream, static_cast<float*>(workspace), gy,
+        hipLaunchKernelGGL(bias_sum_kernel<float>, grid, dim3(1024), 0, stream, static_cast<float*>(workspace), gy,
                            (int)N, static_cast<float*>(db));
       else
-        hipLaunchKernelGGL(bias_sum_kernel<E>, grid, dim3(256), 0, stream, static_cast<float*>(workspace), gy, (int)N,
+        hipLaunchKernelGGL(bias_sum_kernel<E>, grid, dim3(1024), 0, stream, static_cast<float*>(workspace), gy, (int)N,
                            static_cast<E*>(db));
     }
   });

@@ -336,25 +336,12 @@ template <class W>
 __global__ __launch_bounds__(1024) void norm_sum_kernel(const float* __restrict__ part, int n, int cols,
                                                         W* __restrict__ dw, W* __restrict__ db) {
   __shared__ float sum[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t j = (int64_t)blockIdx.x * 64 + lane, pitch = 2 * (int64_t)cols;
-  float a[4] = {};
-  if (j < pitch) {
-    int k = wave;
-    for (; k + 48 < n; k += 64)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) a[u] += part[(k + 16 * u) * pitch + j];
-    for (; k < n; k += 16) a[0] += part[k * pitch + j];
-  }
-  sum[wave][lane] = (a[0] + a[1]) + (a[2] + a[3]);
-  __syncthreads();
-  if (wave == 0 && j < pitch) {
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) s += sum[k][lane];
+  const int64_t j = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = partial_rows_sum(part, n, 2 * (int64_t)cols, j, sum);
+  if (threadIdx.x < 64) {
     if (j < cols) {
       if (dw) dw[j] = (W)s;
-    } else if (db) {
+    } else if (j < 2 * (int64_t)cols && db) {
       db[j - cols] = (W)s;
     }
   }

@@ -77,14 +77,15 @@ def _losses(args: "_lib.DistillArgs", device: torch.device):
     return loss, parts, used
 
 
-def _reduced(loss: torch.Tensor, used: torch.Tensor, reduction: str) -> torch.Tensor:
-    """[2]: the reduced loss and the factor it was multiplied by."""
-    out = torch.empty(2, dtype=torch.float32, device=loss.device)
+def _reduced(loss: torch.Tensor, used: torch.Tensor, reduction: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The reduced loss and the factor it was multiplied by."""
+    out = torch.empty((), dtype=torch.float32, device=loss.device)
+    factor = torch.empty((), dtype=torch.float32, device=loss.device)
     st = _lib.lib().void_distill_reduce(loss.data_ptr(), used.data_ptr(), loss.numel(), reduction == "mean",
-                                        out.data_ptr(), out.data_ptr() + 4, raw_stream(loss.device))
+                                        out.data_ptr(), factor.data_ptr(), raw_stream(loss.device))
     if st:
         _lib.check(st, "void_distill_reduce")
-    return out
+    return out, factor
 
 
 class _Distillation(Function):
@@ -92,22 +93,22 @@ class _Distillation(Function):
     def forward(ctx: Any, logits, teacher, index, temperature, reduction):
         s, t, i, args = _checked(logits, teacher, index, temperature)
         loss, parts, used = _losses(args, s.device)
-        out = None if reduction == "none" else _reduced(loss, used, reduction)
-        ctx.save_for_backward(s, t, i, parts, out)
+        out, factor = (loss.view(logits.shape[:-1]), None) if reduction == "none" else _reduced(loss, used, reduction)
+        ctx.save_for_backward(s, t, i, parts, factor)
         ctx.args, ctx.shape = args, logits.shape
-        return loss.view(logits.shape[:-1]) if out is None else out[0].clone()
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        s, t, i, parts, out = ctx.saved_tensors
+        s, t, i, parts, factor = ctx.saved_tensors
         ds = torch.empty(ctx.shape, dtype=s.dtype, device=s.device)
         if not ds.numel():
             return ds, None, None, None, None
         g = grad.reshape(-1).to(torch.float32)
         st = _lib.lib().void_distill_grad(ctypes.byref(ctx.args), parts.data_ptr(), g.data_ptr(),
-                                          g.stride(0) if out is None else 0,
-                                          out.data_ptr() + 4 if out is not None else None, ds.data_ptr(), s.shape[1],
+                                          g.stride(0) if factor is None else 0,
+                                          factor.data_ptr() if factor is not None else None, ds.data_ptr(), s.shape[1],
                                           raw_stream(s.device))
         if st:
             _lib.check(st, "void_distill_grad")
@@ -130,7 +131,7 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     """
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _runtime.differentiated(logits):
         return _Distillation.apply(logits, teacher_logits, teacher_indices, temperature, reduction)
     s, _, _, args = _checked(logits, teacher_logits, teacher_indices, temperature)
     loss, _, used = _losses(args, s.device)

@@ -185,7 +185,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
             raise ValueError(f"x on {x.device}, {what} on {t.device}")
     if bias is not None:
         bias = (bias if bias.dtype in (x.dtype, torch.float32) else bias.to(torch.float32)).contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _runtime.differentiated(x, weight, bias, residual):
         return _FusedLinear.apply(x, weight, bias, residual, code)
     return _forward(x, weight, bias, residual, code, False)[0]
 

@@ -102,8 +102,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         weight = (weight if weight.dtype in (x.dtype, wide) else weight.to(wide)).contiguous()
     if bias is not None:
         bias = (bias if bias.dtype in (x.dtype, wide) else bias.to(wide)).contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _runtime.differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, float(eps), False)[0]
 
