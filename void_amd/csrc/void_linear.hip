@@ -310,7 +310,7 @@ struct Place {
 
 // ROWS rows x COLS columns of sums from the wave's strip in LDS: whole pieces of
 // rows through the epilogue (or to the partial sums), four of them in flight.
-template <class E, int COLS, int ROWS>
+template <class E, int COLS, int ROWS, int PITCH = COLS>
 __device__ __forceinline__ void store_strip(const Product& p, int split, const float* strip, int64_t row0, int64_t col0,
                                             int lane) {
   constexpr int n = Piece<E>::n, kLanes = COLS / n, kRows = 64 / kLanes, kAhead = ROWS / kRows < 4 ? ROWS / kRows : 4;
@@ -320,7 +320,7 @@ __device__ __forceinline__ void store_strip(const Product& p, int split, const f
   if (col >= N) return;
   float bias[n];
   bias_piece<E>(p.epi, col, N, bias);
-  strip += lane / kLanes * COLS + c;
+  strip += lane / kLanes * PITCH + c;
   row0 += lane / kLanes;
 #pragma unroll 1
   for (int q = 0; q < ROWS; q += kAhead * kRows) {
@@ -328,7 +328,7 @@ __device__ __forceinline__ void store_strip(const Product& p, int split, const f
     typename Piece<E>::vec res[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      z[u] = *reinterpret_cast<const F*>(strip + (q + u * kRows) * COLS);
+      z[u] = *reinterpret_cast<const F*>(strip + (q + u * kRows) * PITCH);
       if (row0 + q + u * kRows < p.M) res[u] = residual_piece<E>(p.epi, row0 + q + u * kRows, col, N);
     }
 #pragma unroll
@@ -607,7 +607,9 @@ __global__ __launch_bounds__(256, 1) void wide_plain_kernel(Product p) {
   }
   wait_vm<0>();     // loads past the last step still write zeros
   __syncthreads();
-  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 64 * 128;
+  // Rows 144 floats apart: the four rows of a store then lie in different banks.
+  constexpr int kPitch = 144;
+  float* strip = reinterpret_cast<float*>(&lds[0][0]) + wave * 64 * kPitch;
   each_of(
       [&](auto h_) {
         constexpr int h = 4 * decltype(h_)::value;
@@ -618,8 +620,8 @@ __global__ __launch_bounds__(256, 1) void wide_plain_kernel(Product p) {
           for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              strip[(16 * i + 4 * (lane >> 4) + r) * 128 + 16 * j + (lane & 15)] = acc[h + i][j][r];
-        store_strip<E, 128, 64>(p, at.split, strip, at.m0 + wm + 16 * h, at.n0 + wn, lane);
+              strip[(16 * i + 4 * (lane >> 4) + r) * kPitch + 16 * j + (lane & 15)] = acc[h + i][j][r];
+        store_strip<E, 128, 64, kPitch>(p, at.split, strip, at.m0 + wm + 16 * h, at.n0 + wn, lane);
       },
       std::make_integer_sequence<int, 2>{});
 }
