@@ -204,32 +204,35 @@ struct Operand {
     return kCpr >= 16 ? (r & 3) << 2 : kCpr == 8 ? (r & 2) << 1 : 0;
   }
 
+  // From load to load a wave's rows go on by kRows, which leaves the permutation as it is.
+  static constexpr int kRows = TURNED ? NW * 64 / kCpr : NW * 8;
+  static_assert(kRows % (TURNED ? 4 : 8) == 0);
+
   const uint8_t* base;  // of the next step's first row / column
   int64_t step;         // bytes from step to step
   int voff[kLoads];
-  int at[kLoads];       // r of the load's chunk within a step
+  int at;               // r of load 0's chunk within a step; turned: kRows more for each next
 
+  // I - i0 rows (turned: columns) remain from i0 on.  Offsets within a step fit 31 bits
+  // (checked by the host).
   __device__ __forceinline__ void init(const void* p, int64_t ld, int64_t i0, int64_t I, int64_t r0, int wave,
                                        int lane) {
+    const int id = wave * 64 + lane, pitch = (int)ld * (int)sizeof(E);
+    const int rows = (int)std::min<int64_t>(I - i0, B);
     if constexpr (!TURNED) {
       base = static_cast<const uint8_t*>(p) + (i0 * ld + r0) * (int64_t)sizeof(E);
       step = 128;
+      const int row = id >> 3, c = (id & 7) ^ (row & 7), first = row * pitch + 16 * c;
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) voff[q] = row + q * kRows < rows ? first + q * kRows * pitch : kOutOfRange;
+      at = c * kPer;
     } else {
       base = static_cast<const uint8_t*>(p) + (r0 * ld + i0) * (int64_t)sizeof(E);
       step = ld * 128;
-    }
+      const int row = id / kCpr, c = (id % kCpr) ^ swizzle(row), first = row * pitch + 16 * c;
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
-      const int id = (q * NW + wave) * 64 + lane;
-      if constexpr (!TURNED) {
-        const int row = id >> 3, c = (id & 7) ^ (row & 7);
-        voff[q] = i0 + row < I ? (int)(row * ld * (int64_t)sizeof(E)) + 16 * c : kOutOfRange;
-        at[q] = c * kPer;
-      } else {
-        const int row = id / kCpr, c = (id % kCpr) ^ swizzle(row);
-        voff[q] = i0 + c * kPer < I ? (int)(row * ld * (int64_t)sizeof(E)) + 16 * c : kOutOfRange;
-        at[q] = row;
-      }
+      for (int q = 0; q < kLoads; ++q) voff[q] = c * kPer < rows ? first + q * kRows * pitch : kOutOfRange;
+      at = row;
     }
   }
 
@@ -237,7 +240,7 @@ struct Operand {
   // of r remain from it on.
   template <int Q>
   __device__ __forceinline__ void load_one(uint8_t* lds, int wave, int left) {
-    dma_b128(sgpr_rsrc(base), lds + (Q * NW + wave) * 1024, at[Q] < left ? voff[Q] : kOutOfRange, 0);
+    dma_b128(sgpr_rsrc(base), lds + (Q * NW + wave) * 1024, at + (TURNED ? Q * kRows : 0) < left ? voff[Q] : kOutOfRange, 0);
     if (Q == kLoads - 1) base += step;
   }
   template <int... Q>
