@@ -17,14 +17,13 @@
 // gradient is rounded once.  A row's entries live in LDS; one wave makes their
 // probabilities, the loss and their logits' few gradients, which it writes again,
 // with the p of equal indices added in order, behind the barrier that follows the
-// row's (no atomics).
+// row's gradient (no atomics).
 //
 // Many rows: one workgroup of T threads a row.  Few rows: S slices of each row,
 // whose (m, z) parts every reader joins for itself in slice order.  Loss and
 // gradient in one call keep what they can of a row in registers between the sum and
 // the gradient and read the rest again while it is in the caches: one read of the
-// memory, one write.  Measured, 8192 x 131072 bf16 with a quarter of the rows without
-// entries: 810 to 880 us, 4.3 to 4.65 TB/s of those bytes (a copy of 2 GiB: 4.94).
+// memory, one write.
 
 #include <hip/hip_runtime.h>
 
@@ -126,15 +125,16 @@ struct Entries {
   int32_t* at;  // index, -1 where the entry does not count
   float* t;     // the teacher's logit, later its probability
   float* s;     // the student's logit there
+  float* w;     // the probabilities of all entries of its index; -1 unless it is the first of them
 };
 
 constexpr int pad4(int k) { return (k + 3) & ~3; }
 
 __device__ __forceinline__ Entries entries_of(float* lds, int k) {
-  return Entries{reinterpret_cast<int32_t*>(lds), lds + pad4(k), lds + 2 * pad4(k)};
+  return Entries{reinterpret_cast<int32_t*>(lds), lds + pad4(k), lds + 2 * pad4(k), lds + 3 * pad4(k)};
 }
 
-size_t entries_bytes(int k) { return (size_t)pad4(std::max(k, 1)) * 12; }
+size_t entries_bytes(int k) { return (size_t)pad4(std::max(k, 1)) * 16; }
 
 __device__ __forceinline__ int64_t entry_index(const Args& a, int64_t row, int j) {
   return a.index_bytes == 8 ? static_cast<const int64_t*>(a.index)[row * a.ldi + j]
@@ -150,13 +150,11 @@ __device__ __forceinline__ float entry_logit(const Args& a, int64_t row, int j) 
 
 __device__ __forceinline__ bool entry_counts(int64_t at, float t) { return at >= 0 && !(t == -INFINITY); }
 
-// All that a row's entries ask for, by one wave (the others go on): p, the loss
-// (returned) from m and z = sum exp2((s - m) c), and, unless ds is null, the
-// gradients of the entries' logits with index in [lo, hi), where the first of equal
-// indices writes, with all their p.  Everything else of the gradient is written.
-template <class E>
-__device__ __forceinline__ float entries_by_wave(const Args& a, const Entries& en, int flags, float m, float z, float gs,
-                                                 int64_t lo, int64_t hi, E* ds) {
+// What a row's entries ask for, by one wave (the others go on), in two parts.  The
+// first needs the teacher alone: p and, where the gradient is made, the p of equal
+// indices, which the first of them takes.  Returns the lane's part of sum p log p.
+__device__ __forceinline__ float teacher_by_wave(const Args& a, const Entries& en, int flags, int64_t lo,
+                                                 int64_t hi) {
   const int lane = threadIdx.x & 63;
   float top = -INFINITY;
   for (int j = lane; j < a.k; j += 64)
@@ -170,37 +168,53 @@ __device__ __forceinline__ float entries_by_wave(const Args& a, const Entries& e
   for (int j = lane; j < a.k; j += 64)
     if (en.at[j] >= 0) sum += pow2((en.t[j] - top) * a.c);
   sum = flags & kBad ? NAN : lanes_sum<64>(sum);
-  const float inv = 1.f / sum, back = logf(z) - logf(sum);
-  float loss = 0.f;
+  const float inv = 1.f / sum, log_sum = logf(sum);
+  float own = 0.f;
   for (int j = lane; j < a.k; j += 64) {
     const float d = en.t[j] - top, p = en.at[j] >= 0 ? pow2(d * a.c) * inv : 0.f;
-    // log p - log q = (t - top) / T - log sum - (s - m) / T + log z
-    if (p != 0.f) loss += p * ((d - (en.s[j] - m)) / a.temperature + back);
+    if (p != 0.f) own += p * (d / a.temperature - log_sum);  // log p
     en.t[j] = p;
   }
-  loss = lanes_sum<64>(loss) * a.temperature * a.temperature;
-  if (ds) {
-    const float iz = 1.f / z;
-    for (int j = lane; j < a.k; j += 64) {
-      const int at = en.at[j];
-      if (at < lo || at >= hi) continue;
-      float p = 0.f;
-      bool first = true;
-      for (int i = 0; i < a.k; i += 4) {
-        const int4 q = *reinterpret_cast<const int4*>(en.at + i);
-        if (q.x == at || q.y == at || q.z == at || q.w == at) {
+  for (int j = lane; j < a.k; j += 64) {
+    const int at = en.at[j];
+    if (at < lo || at >= hi) continue;
+    float p = 0.f;
+    bool first = true;
+    for (int i = 0; i < a.k; i += 4) {
+      const int4 q = *reinterpret_cast<const int4*>(en.at + i);
+      if (q.x == at || q.y == at || q.z == at || q.w == at) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if ((e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w) == at) {
-              first &= i + e >= j;
-              p += en.t[i + e];
-            }
-        }
+        for (int e = 0; e < 4; ++e)
+          if ((e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w) == at) {
+            first &= i + e >= j;
+            p += en.t[i + e];
+          }
       }
-      if (first) ds[at] = (E)(gs * (pow2((en.s[j] - m) * a.c) * iz - p));
+    }
+    en.w[j] = first ? p : -1.f;
+  }
+  return own;
+}
+
+// The second needs m and z = sum exp2((s - m) c): the loss (returned) and, unless ds
+// is null, the gradients of the entries' logits with index in [lo, hi), behind a
+// barrier that follows everything else of the row's gradient.
+template <class E>
+__device__ __forceinline__ float entries_by_wave(const Args& a, const Entries& en, float own, float m, float z, float gs,
+                                                 int64_t lo, int64_t hi, E* ds) {
+  const int lane = threadIdx.x & 63;
+  const float back = logf(z), iz = 1.f / z;
+  float loss = own;
+  for (int j = lane; j < a.k; j += 64) {
+    const float p = en.t[j], d = en.s[j] - m;
+    if (p != 0.f) loss += p * (back - d / a.temperature);  // - log q
+    if (ds) {
+      const int at = en.at[j];
+      const float w = en.w[j];
+      if (at >= lo && at < hi && !(w < 0.f)) ds[at] = (E)(gs * (pow2(d * a.c) * iz - w));
     }
   }
-  return loss;
+  return lanes_sum<64>(loss) * a.temperature * a.temperature;
 }
 
 // ---- slices of a row ---------------------------------------------------------
@@ -271,14 +285,13 @@ __device__ __forceinline__ Part slice_part(const Args& a, const E* s, const Slic
   return Part{top, z};
 }
 
-// The S parts of a row joined; a wave at a time, every wave the same.
-__device__ __forceinline__ Part join_parts(const float2* parts, int S, float c) {
+// The S parts of a row, one a lane, and joined; a wave at a time, every wave the same.
+__device__ __forceinline__ Part lane_part(const float2* parts, int S) {
   const int lane = threadIdx.x & 63;
-  Part p{kLowest, 0.f};
-  if (lane < S) {
-    const float2 f = parts[lane];
-    p = Part{f.x, f.y};
-  }
+  const float2 f = lane < S ? parts[lane] : make_float2(kLowest, 0.f);
+  return Part{f.x, f.y};
+}
+__device__ __forceinline__ Part join_parts(Part p, int S, float c) {
   if (S > 1)
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) p = join(p, Part{__shfl_xor(p.m, off, 64), __shfl_xor(p.z, off, 64)}, c);
@@ -320,7 +333,9 @@ __device__ __forceinline__ int take_entries(const Args& a, int64_t row, const E*
 // ---- kernels ---------------------------------------------------------------
 
 // Unit u = (row, slice).  Writes the slice's part; used[row] (slice 0).  With
-// LOSS (S = 1) the row's loss too.
+// LOSS (S = 1) the row's loss too.  Bound by reading the logits: 4096 x 32768 bf16
+// 52 us, 5.2 TB/s; 730 x 50021 fp32 with a quarter of the rows without entries 24 us,
+// 4.5 TB/s.
 template <class E, int T, bool LOSS>
 __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t units, float2* __restrict__ parts,
                                                           int32_t* __restrict__ used, float* __restrict__ loss) {
@@ -346,7 +361,9 @@ __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t
     if (flags & kSome) p = slice_part<E, T>(a, s, Slice<E>(a.vocab, S, sl), red);
     if (threadIdx.x < 64) {
       float l = 0.f;
-      if (LOSS && flags & kSome) l = entries_by_wave<E>(a, en, flags, p.m, p.z, 0.f, 0, 0, nullptr);
+      if constexpr (LOSS)
+        if (flags & kSome)
+          l = entries_by_wave<E>(a, en, teacher_by_wave(a, en, flags, 0, 0), p.m, p.z, 0.f, 0, 0, nullptr);
       if (threadIdx.x == 0) {
         parts[u] = make_float2(p.m, p.z);
         if (sl == 0) used[row] = flags & kSome;
@@ -368,8 +385,8 @@ __global__ __launch_bounds__(64) void distill_loss_kernel(Args a, int S, const f
     float l = 0.f;
     const int flags = take_entries<E, 64>(a, row, static_cast<const E*>(a.logits) + row * a.ld, en, red);
     if (flags & kSome) {
-      const Part p = join_parts(parts + row * S, S, a.c);
-      l = entries_by_wave<E>(a, en, flags, p.m, p.z, 0.f, 0, 0, nullptr);
+      const Part p = join_parts(lane_part(parts + row * S, S), S, a.c);
+      l = entries_by_wave<E>(a, en, teacher_by_wave(a, en, flags, 0, 0), p.m, p.z, 0.f, 0, 0, nullptr);
     }
     if (threadIdx.x == 0) loss[row] = l;
   }
@@ -387,7 +404,10 @@ __device__ __forceinline__ float total_count(const int32_t* counts, int n) {
 // Gradient, unit u = (row, slice) of G.  The upstream gradient is g[row * gstep],
 // times *factor where that is not null, times scale; `counts` (n of them, or
 // null) divides by the number of rows with entries.  With `loss`, slice 0
-// writes the row's loss.
+// writes the row's loss.  Bound by one read of the logits and one write of as much:
+// 4096 x 32768 bf16 102 us, 5.3 TB/s; 730 x 50021 fp32 with a quarter of the rows
+// without entries 58 us, 4.4 TB/s.  What the entries need of the teacher is made while
+// the logits come (300 x 131072 bf16, loss and gradient: 50.4 us, and 54.4 at the end).
 template <class E, int T>
 __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const float2* __restrict__ parts, int G,
                                                          int64_t units, const float* __restrict__ g, int64_t gstep,
@@ -409,20 +429,27 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
     const Slice<E> sl(a.vocab, G, n);
     const E* s = static_cast<const E*>(a.logits) + row * a.ld;
     E* ds = grad + row * ldg;
+    const Part mine = lane_part(parts + row * S, S);
     const int flags = take_entries<E, T>(a, row, s, en, red);
     if (!(flags & kSome)) {
       zero_slice<E, T>(ds, sl);
       if (loss && n == 0 && threadIdx.x == 0) loss[row] = 0.f;
       continue;
     }
-    const Part st = join_parts(parts + row * S, S, a.c);
     const float gs = (g ? g[row * gstep] * scale : scale) * a.temperature;
-    const float f = flags & kBad ? NAN : gs / st.z;
-    for (uint32_t q = sl.first + threadIdx.x; q < sl.last; q += kAhead * T) {
-      V v[kAhead];
+    V v[kAhead];
+    auto load = [&](uint32_t q) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (q + i * T < sl.last) v[i] = *reinterpret_cast<const Any*>(s + (int64_t)(q + i * T) * N);
+    };
+    uint32_t q = sl.first + threadIdx.x;
+    load(q);
+    float own = 0.f;
+    if (threadIdx.x < 64) own = teacher_by_wave(a, en, flags, sl.lo, sl.hi);  // while they come
+    const Part st = join_parts(mine, S, a.c);
+    const float f = flags & kBad ? NAN : gs / st.z;
+    while (q < sl.last) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (q + i * T < sl.last) {
@@ -431,6 +458,8 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
           for (int e = 0; e < N; ++e) o[e] = pow2((o[e] - st.m) * a.c) * f;
           stream_out(ds + (int64_t)(q + i * T) * N, __builtin_convertvector(o, V));
         }
+      q += kAhead * T;
+      load(q);
     }
     if (threadIdx.x < sl.rest) {
       const int64_t c = (int64_t)sl.last * N + threadIdx.x;
@@ -438,7 +467,7 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
     }
     __syncthreads();  // the entries' logits are written again
     if (threadIdx.x < 64) {
-      const float l = entries_by_wave<E>(a, en, flags, st.m, st.z, gs, sl.lo, sl.hi, ds);
+      const float l = entries_by_wave<E>(a, en, own, st.m, st.z, gs, sl.lo, sl.hi, ds);
       if (loss && n == 0 && threadIdx.x == 0) loss[row] = l;
     }
   }
@@ -470,7 +499,9 @@ __global__ __launch_bounds__(1024) void distill_count_kernel(Args a, int32_t* __
 // Loss and gradient of whole rows.  The first NV pieces a thread of a row stay in
 // registers between its sums and its gradient; what a longer row has behind them is
 // read again from the caches.  Four waves a SIMD: while one workgroup sums, others
-// load and store.
+// load and store.  Bound by the memory: 8192 x 65536 bf16 466 us, 4.6 TB/s of one read
+// and one write; x 131072 967 us, 4.45, with a quarter of the rows without entries
+// 820 to 870 us, 4.3 to 4.6 (a copy of 2 GiB: 4.94).
 template <class E, int T, int NV>
 __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale, const int32_t* __restrict__ counts,
                                                             int n_counts, E* __restrict__ grad, int64_t ldg,
@@ -593,8 +624,11 @@ __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale,
     }
     if (threadIdx.x < rest) ds[(int64_t)whole * N + threadIdx.x] = (E)(pow2((tail - m) * a.c) * f0);
     __syncthreads();  // the entries' logits are written again
+    // Both parts here: the other waves end now and make room for the next row's (with
+    // the first part before the barrier 8192 x 16384 bf16 139 us against 125).
     if (threadIdx.x < 64) {
-      const float l = entries_by_wave<E>(a, en, flags, m, z, gs, 0, a.vocab, ds);
+      const float own = teacher_by_wave(a, en, flags, 0, a.vocab);
+      const float l = entries_by_wave<E>(a, en, own, m, z, gs, 0, a.vocab, ds);
       if (threadIdx.x == 0) loss[row] = l;
     }
   }
@@ -650,9 +684,11 @@ int slices(int64_t rows, int vocab) {
 // go(T) for slices of `pieces` 16-byte pieces: few threads a slice, since each
 // workgroup has its entries to see to (gradient of 8192 rows bf16: 2000 wide 19 us with
 // 64 threads, 31 with 256; 8192 wide 60 and 52; 2048 x 131072 216 with 256, 208 with 512).
+// With `few` rows to fill the chip 256 at least (loss and gradient of one row x 131072
+// 13.3 us, and 14.4 with 64).
 template <class Go>
-void by_length(int64_t pieces, Go go) {
-  if (pieces <= 512) go(std::integral_constant<int, 64>{});
+void by_length(int64_t pieces, bool few, Go go) {
+  if (!few && pieces <= 512) go(std::integral_constant<int, 64>{});
   else if (pieces <= 8192) go(std::integral_constant<int, 256>{});
   else go(std::integral_constant<int, 512>{});
 }
@@ -698,7 +734,7 @@ Args args_of(const void_distill_args* d) {
 template <class E>
 void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, hipStream_t stream) {
   const int64_t units = a.rows * S;
-  by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, [&](auto t) {
+  by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, S > 1, [&](auto t) {
     constexpr int T = decltype(t)::value;
     const dim3 grid((unsigned)std::min(units, kMaxGrid));
     if (S == 1 && loss)
@@ -715,7 +751,7 @@ template <class E>
 void gradient(const Args& a, int S, const float2* part, const float* g, int64_t gstep, const float* factor, float scale,
               const int32_t* counts, int n_counts, void* grad, int64_t ldg, float* loss, hipStream_t stream) {
   const int64_t units = a.rows * S;
-  by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, [&](auto t) {
+  by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, S > 1, [&](auto t) {
     constexpr int T = decltype(t)::value;
     hipLaunchKernelGGL((distill_grad_kernel<E, T>), dim3((unsigned)std::min(units, kMaxGrid)), dim3(T), entries_bytes(a.k), stream, a, S,
                        part, S, units, g, gstep, factor, scale, counts, n_counts, static_cast<E*>(grad), ldg, loss);
