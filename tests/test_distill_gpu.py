@@ -278,6 +278,25 @@ def test_streams_and_graphs(gpu):
 
 
 @gpu_only
+@pytest.mark.parametrize("R,V", [(1, 9000), (15, 20001), (16, 40000), (17, 40000), (40, 9000)])
+def test_few_rows_give_the_same_sum_each_time(gpu, R, V):
+    s, t, idx = inputs(gpu, R, V, 33, torch.bfloat16, seed=R, ragged=True)
+    idx[0] = -1  # a row that does not count arrives too
+    check(s, t, idx, 2.0)
+    want = void_amd.distillation_loss_and_grad(s, t, idx)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = void_amd.distillation_loss_and_grad(s, t, idx)
+    for _ in range(5):
+        got[0].fill_(7.0), got[1].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        again = void_amd.distillation_loss_and_grad(s, t, idx)
+        for out in (got, again):
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@gpu_only
 def test_forward_mode_and_second_derivatives_are_refused(gpu):
     from torch.autograd import forward_ad
     with forward_ad.dual_level():

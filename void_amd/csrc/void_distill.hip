@@ -333,15 +333,17 @@ __device__ __forceinline__ int take_entries(const Args& a, int64_t row, const E*
 // ---- kernels ---------------------------------------------------------------
 
 // Unit u = (row, slice).  Writes the slice's part; used[row] (slice 0).  With
-// LOSS (S = 1) the row's loss too.  Bound by reading the logits: 4096 x 32768 bf16
+// LOSS (S = 1) the row's loss too.  Clears `arrived` (unless null).  Bound by reading the logits: 4096 x 32768 bf16
 // 52 us, 5.2 TB/s; 730 x 50021 fp32 with a quarter of the rows without entries 24 us,
 // 4.5 TB/s.
 template <class E, int T, bool LOSS>
 __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t units, float2* __restrict__ parts,
-                                                          int32_t* __restrict__ used, float* __restrict__ loss) {
+                                                          int32_t* __restrict__ used, float* __restrict__ loss,
+                                                          int32_t* __restrict__ arrived) {
   __shared__ Areas red;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const Entries en = entries_of(lds, a.k);
+  if (arrived && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t row = u / S;
     const int sl = (int)(u - row * S);
@@ -401,10 +403,32 @@ __device__ __forceinline__ float total_count(const int32_t* counts, int n) {
   return (float)c;
 }
 
+// A row's loss by one wave.  With `total` the wave that is last to come (the rows' count
+// of them is in `arrived`) sums all losses in a fixed order, times `share`.
+__device__ __forceinline__ void add_row_loss(const Args& a, int64_t row, float l, float* loss, float share,
+                                             float* total, int32_t* arrived) {
+  const int lane = threadIdx.x & 63;
+  if (!total) {
+    if (lane == 0) loss[row] = l;
+    return;
+  }
+  int before = 0;
+  if (lane == 0) {
+    __hip_atomic_store(loss + row, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    before = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (__shfl(before, 0, 64) != (int)a.rows - 1) return;
+  float s = 0.f;
+  for (int64_t r = lane; r < a.rows; r += 64)
+    s += __hip_atomic_load(loss + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  s = lanes_sum<64>(s);
+  if (lane == 0) *total = s * share;
+}
+
 // Gradient, unit u = (row, slice) of G.  The upstream gradient is g[row * gstep],
 // times *factor where that is not null, times scale; `counts` (n of them, or
 // null) divides by the number of rows with entries.  With `loss`, slice 0
-// writes the row's loss.  Bound by one read of the logits and one write of as much:
+// writes the row's loss; `total` (unless null) becomes their sum or mean.  Bound by one read of the logits and one write of as much:
 // 4096 x 32768 bf16 102 us, 5.3 TB/s; 730 x 50021 fp32 with a quarter of the rows
 // without entries 58 us, 4.4 TB/s.  What the entries need of the teacher is made while
 // the logits come (300 x 131072 bf16, loss and gradient: 50.4 us, and 54.4 at the end).
@@ -413,7 +437,8 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
                                                          int64_t units, const float* __restrict__ g, int64_t gstep,
                                                          const float* __restrict__ factor, float scale,
                                                          const int32_t* __restrict__ counts, int n_counts,
-                                                         E* __restrict__ grad, int64_t ldg, float* __restrict__ loss) {
+                                                         E* __restrict__ grad, int64_t ldg, float* __restrict__ loss,
+                                                         float* __restrict__ total, int32_t* __restrict__ arrived) {
   constexpr int N = Piece<E>::n, kAhead = 4;
   typedef typename Piece<E>::vec V;
   typedef typename Piece<E>::any Any;
@@ -422,7 +447,8 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const Entries en = entries_of(lds, a.k);
   if (factor) scale *= *factor;
-  if (counts) scale /= fmaxf(total_count(counts, n_counts), 1.f);
+  const float share = counts ? 1.f / fmaxf(total_count(counts, n_counts), 1.f) : 1.f;
+  scale *= share;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t row = u / G;
     const int n = (int)(u - row * G);
@@ -433,7 +459,7 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
     const int flags = take_entries<E, T>(a, row, s, en, red);
     if (!(flags & kSome)) {
       zero_slice<E, T>(ds, sl);
-      if (loss && n == 0 && threadIdx.x == 0) loss[row] = 0.f;
+      if (loss && n == 0 && threadIdx.x < 64) add_row_loss(a, row, 0.f, loss, share, total, arrived);
       continue;
     }
     const float gs = (g ? g[row * gstep] * scale : scale) * a.temperature;
@@ -468,7 +494,7 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
     __syncthreads();  // the entries' logits are written again
     if (threadIdx.x < 64) {
       const float l = entries_by_wave<E>(a, en, own, st.m, st.z, gs, sl.lo, sl.hi, ds);
-      if (loss && n == 0 && threadIdx.x == 0) loss[row] = l;
+      if (loss && n == 0) add_row_loss(a, row, l, loss, share, total, arrived);
     }
   }
 }
@@ -732,15 +758,16 @@ Args args_of(const void_distill_args* d) {
 }
 
 template <class E>
-void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, hipStream_t stream) {
+void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, int32_t* arrived,
+           hipStream_t stream) {
   const int64_t units = a.rows * S;
   by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, S > 1, [&](auto t) {
     constexpr int T = decltype(t)::value;
     const dim3 grid((unsigned)std::min(units, kMaxGrid));
     if (S == 1 && loss)
-      hipLaunchKernelGGL((distill_parts_kernel<E, T, true>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss);
+      hipLaunchKernelGGL((distill_parts_kernel<E, T, true>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss, arrived);
     else
-      hipLaunchKernelGGL((distill_parts_kernel<E, T, false>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss);
+      hipLaunchKernelGGL((distill_parts_kernel<E, T, false>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss, arrived);
   });
   if (S > 1 && loss)
     hipLaunchKernelGGL(distill_loss_kernel<E>, dim3((unsigned)std::min(a.rows, kMaxGrid)), dim3(64), entries_bytes(a.k), stream, a, S,
@@ -749,12 +776,13 @@ void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, hipSt
 
 template <class E>
 void gradient(const Args& a, int S, const float2* part, const float* g, int64_t gstep, const float* factor, float scale,
-              const int32_t* counts, int n_counts, void* grad, int64_t ldg, float* loss, hipStream_t stream) {
+              const int32_t* counts, int n_counts, void* grad, int64_t ldg, float* loss, float* total, int32_t* arrived,
+              hipStream_t stream) {
   const int64_t units = a.rows * S;
   by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, S > 1, [&](auto t) {
     constexpr int T = decltype(t)::value;
     hipLaunchKernelGGL((distill_grad_kernel<E, T>), dim3((unsigned)std::min(units, kMaxGrid)), dim3(T), entries_bytes(a.k), stream, a, S,
-                       part, S, units, g, gstep, factor, scale, counts, n_counts, static_cast<E*>(grad), ldg, loss);
+                       part, S, units, g, gstep, factor, scale, counts, n_counts, static_cast<E*>(grad), ldg, loss, total, arrived);
   });
 }
 
@@ -777,6 +805,11 @@ void by_row(int vocab, Go go) {
 
 constexpr int kCountGrid = 256;
 
+// Up to so many rows the gradient's kernel sums the losses itself, a launch less: 8 rows
+// x 131072 bf16 12.7 us against 14.2 (15.2 and 18.2 with the host's part).  Each row that
+// arrives writes an L2 back, so that more rows lose by it: 64 of the same 27 us and 19.5.
+constexpr int64_t kJoinedRows = 16;
+
 int count_grid(int64_t rows) { return (int)std::min<int64_t>((rows + 15) / 16, kCountGrid); }
 
 }  // namespace
@@ -792,7 +825,8 @@ int void_distill_loss(const void_distill_args* d, float* row_loss, float* parts_
   if (!row_loss || !parts_ || !used || (uintptr_t)parts_ % 8) return void_internal_fail(VOID_ERR_ARG, "null output");
   const Args a = args_of(d);
   by_type(d->dtype, [&](auto e) {
-    parts<decltype(e)>(a, slices(d->rows, d->vocab), reinterpret_cast<float2*>(parts_), used, row_loss, stream);
+    parts<decltype(e)>(a, slices(d->rows, d->vocab), reinterpret_cast<float2*>(parts_), used, row_loss, nullptr,
+                       stream);
   });
   return launched();
 }
@@ -816,14 +850,14 @@ int void_distill_grad(const void_distill_args* d, const float* parts_, const flo
   const Args a = args_of(d);
   by_type(d->dtype, [&](auto e) {
     gradient<decltype(e)>(a, slices(d->rows, d->vocab), reinterpret_cast<const float2*>(parts_), upstream,
-                          upstream_step, factor, 1.f, nullptr, 0, grad, ldg, nullptr, stream);
+                          upstream_step, factor, 1.f, nullptr, 0, grad, ldg, nullptr, nullptr, nullptr, stream);
   });
   return launched();
 }
 
 size_t void_distill_step_workspace_bytes(int64_t rows, int32_t vocab) {
   if (rows <= 0) return 0;
-  // Parts (8 bytes each), then a loss and a flag per row and the counts.
+  // Parts (8 bytes each), then a loss and a flag per row and the counts (of the arrived, for few rows).
   return (size_t)rows * slices(rows, vocab) * 8 + (size_t)rows * 8 + kCountGrid * 4;
 }
 
@@ -845,6 +879,9 @@ int void_distill_step(const void_distill_args* d, int32_t mean, float grad_scale
   float* row_loss = reinterpret_cast<float*>(part + d->rows * S);
   int32_t* used = reinterpret_cast<int32_t*>(row_loss + d->rows);
   int32_t* counts = used + d->rows;
+  auto sum = [&] {
+    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, stream, row_loss, used, d->rows, mean, loss, nullptr);
+  };
   by_type(d->dtype, [&](auto e) {
     using E = decltype(e);
     if (S == 1) {
@@ -855,14 +892,16 @@ int void_distill_step(const void_distill_args* d, int32_t mean, float grad_scale
         hipLaunchKernelGGL((distill_step_kernel<E, T, NV>), dim3((unsigned)std::min(d->rows, kMaxGrid)), dim3(T), entries_bytes(a.k), stream, a, grad_scale, mean ? counts : nullptr, n,
                            static_cast<E*>(grad), ldg, row_loss, used);
       });
+      sum();
       return;
     }
-    // Few rows: the parts of their slices, then the gradient (and each row's loss).
-    parts<E>(a, S, part, used, nullptr, stream);
+    // Few rows: the parts of their slices, then the gradient and each row's loss.
+    const bool join = d->rows <= kJoinedRows;
+    parts<E>(a, S, part, used, nullptr, join ? counts : nullptr, stream);
     gradient<E>(a, S, part, nullptr, 0, nullptr, grad_scale, mean ? used : nullptr, (int)d->rows, grad, ldg, row_loss,
-                stream);
+                join ? loss : nullptr, counts, stream);
+    if (!join) sum();
   });
-  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, stream, row_loss, used, d->rows, mean, loss, nullptr);
   return launched();
 }
 

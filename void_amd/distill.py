@@ -152,7 +152,7 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tenso
     R, V = s.shape
     lib = _lib.lib()
     loss = torch.empty((), dtype=torch.float32, device=s.device)
-    grad = torch.empty(logits.shape, dtype=s.dtype, device=s.device)
+    grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
     ws = torch.empty(lib.void_distill_step_workspace_bytes(R, V), dtype=torch.uint8, device=s.device)
     st = lib.void_distill_step(ctypes.byref(args), reduction == "mean", float(grad_scale), loss.data_ptr(),
                                grad.data_ptr(), V, ws.data_ptr(), ws.numel(), raw_stream(s.device))

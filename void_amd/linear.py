@@ -64,7 +64,7 @@ def _forward(x, weight, bias, residual, code: int, with_slope: bool):
     else:
         rows, w = _runtime.padded_rows(rows, zero_tail=True), _runtime.padded_rows(weight, zero_tail=True)
         depth = _whole(K, x)
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape[:-1] + (N,))
     slope = None
     if with_slope:
         slope = torch.empty(M, N, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16, device=x.device)

@@ -24,7 +24,7 @@ def _forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[tor
     """(y, the rows x was read as, their statistics or None)."""
     rows = _runtime.flat_rows(x)
     R, C = rows.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty(R, 2, dtype=torch.float32, device=x.device) if with_stats else None
     param = weight if weight is not None else bias
     st = _lib.lib().void_layer_norm(
