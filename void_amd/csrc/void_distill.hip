@@ -428,10 +428,11 @@ __device__ __forceinline__ void add_row_loss(const Args& a, int64_t row, float l
 // Gradient, unit u = (row, slice) of G.  The upstream gradient is g[row * gstep],
 // times *factor where that is not null, times scale; `counts` (n of them, or
 // null) divides by the number of rows with entries.  With `loss`, slice 0
-// writes the row's loss; `total` (unless null) becomes their sum or mean.  Bound by one read of the logits and one write of as much:
-// 4096 x 32768 bf16 102 us, 5.3 TB/s; 730 x 50021 fp32 with a quarter of the rows
-// without entries 58 us, 4.4 TB/s.  What the entries need of the teacher is made while
-// the logits come (300 x 131072 bf16, loss and gradient: 50.4 us, and 54.4 at the end).
+// writes the row's loss; `total` (unless null) becomes their sum or mean.  Bound by
+// one read of the logits and one write of as much: 4096 x 32768 bf16 102 us, 5.3 TB/s;
+// 730 x 50021 fp32 with a quarter of the rows without entries 58 us, 4.4 TB/s.  What
+// the entries need of the teacher is made while the logits come (300 x 131072 bf16,
+// loss and gradient: 50.4 us, and 54.4 at the end).
 template <class E, int T>
 __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const float2* __restrict__ parts, int G,
                                                          int64_t units, const float* __restrict__ g, int64_t gstep,
@@ -765,9 +766,11 @@ void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, int32
     constexpr int T = decltype(t)::value;
     const dim3 grid((unsigned)std::min(units, kMaxGrid));
     if (S == 1 && loss)
-      hipLaunchKernelGGL((distill_parts_kernel<E, T, true>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss, arrived);
+      hipLaunchKernelGGL((distill_parts_kernel<E, T, true>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part,
+                         used, loss, arrived);
     else
-      hipLaunchKernelGGL((distill_parts_kernel<E, T, false>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part, used, loss, arrived);
+      hipLaunchKernelGGL((distill_parts_kernel<E, T, false>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part,
+                         used, loss, arrived);
   });
   if (S > 1 && loss)
     hipLaunchKernelGGL(distill_loss_kernel<E>, dim3((unsigned)std::min(a.rows, kMaxGrid)), dim3(64), entries_bytes(a.k), stream, a, S,
