@@ -19,6 +19,7 @@ from typing import Dict, List, Optional, Tuple
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import _lib, tuning
 from ._streams import raw_stream, record_once
@@ -75,6 +76,16 @@ def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
     operator does not take."""
     return forward_ad._current_level >= 0 or (torch.is_grad_enabled()
                                               and any(t is not None and t.requires_grad for t in tensors))
+
+
+def first_order(backward):
+    """once_differentiable for a backward pass, without its cost (a guard around
+    every call) where autograd records no graph of the gradient anyway."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def flat_rows(t: torch.Tensor) -> torch.Tensor:

@@ -22,7 +22,6 @@ from typing import Any, Tuple
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _runtime
 from ._streams import raw_stream
@@ -99,10 +98,10 @@ class _Distillation(Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
         s, t, i, parts, factor = ctx.saved_tensors
-        ds = torch.empty(ctx.shape, dtype=s.dtype, device=s.device)
+        ds = s.new_empty(ctx.shape)
         if not ds.numel():
             return ds, None, None, None, None
         g = grad.reshape(-1).to(torch.float32)

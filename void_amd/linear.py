@@ -19,7 +19,6 @@ from typing import Any, Optional, Union
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _runtime
 from ._streams import raw_stream
@@ -108,7 +107,7 @@ class _FusedLinear(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
         rows, w, slope = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad

@@ -9,11 +9,11 @@ Statistics are fp32 whatever x's type; y and the gradients are rounded once.
 
 from __future__ import annotations
 
+import functools
 from typing import Any, Optional
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _runtime
 from ._streams import raw_stream
@@ -37,36 +37,40 @@ def _forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[tor
     return y, rows, stats
 
 
+@functools.lru_cache(maxsize=256)
+def _grad_workspace_bytes(R: int, C: int, code: int) -> int:
+    return _lib.lib().void_layer_norm_grad_workspace_bytes(R, C, code)
+
+
 class _LayerNorm(Function):
     @staticmethod
     def forward(ctx: Any, x, weight, bias, eps):
         y, rows, stats = _forward(x, weight, bias, eps, True)
         ctx.save_for_backward(rows, weight, stats)
-        ctx.shape, ctx.bias_dtype = x.shape, None if bias is None else bias.dtype
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
     @staticmethod
-    @once_differentiable
+    @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
         rows, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         R, C = rows.shape
         dy = _runtime.flat_rows(grad)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = rows.device
-        dx = torch.empty(ctx.shape, dtype=rows.dtype, device=dev) if need_x else None
-        dtype = weight.dtype if weight is not None else ctx.bias_dtype or rows.dtype
-        dw = torch.empty(C, dtype=dtype, device=dev) if need_w else None
-        db = torch.empty(C, dtype=dtype, device=dev) if need_b else None
-        lib, code = _lib.lib(), _runtime.FLOAT_CODES[rows.dtype]
-        ws = None
+        dx = torch.empty_like(grad, memory_format=torch.contiguous_format) if need_x else None
+        param = weight if weight is not None else rows.new_empty(C, dtype=ctx.bias_dtype or rows.dtype)
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(param) if need_b else None
+        code, ws, ws_bytes = _runtime.FLOAT_CODES[rows.dtype], None, 0
         if need_w or need_b:
-            ws = torch.empty(lib.void_layer_norm_grad_workspace_bytes(R, C, code), dtype=torch.uint8, device=dev)
-        st = lib.void_layer_norm_grad(
+            ws_bytes = _grad_workspace_bytes(R, C, code)
+            ws = stats.new_empty(ws_bytes // 4)
+        st = _lib.lib().void_layer_norm_grad(
             dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0),
-            weight.data_ptr() if weight is not None else None, _runtime.FLOAT_CODES[dtype], stats.data_ptr(), R, C, code,
-            dx.data_ptr() if need_x else None, C, dw.data_ptr() if need_w else None,
-            db.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None,
-            ws.numel() if ws is not None else 0, raw_stream(dev))
+            weight.data_ptr() if weight is not None else None, _runtime.FLOAT_CODES[param.dtype], stats.data_ptr(), R, C,
+            code, dx.data_ptr() if need_x else None, C, dw.data_ptr() if need_w else None,
+            db.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None, ws_bytes,
+            raw_stream(rows.device))
         if st:
             _lib.check(st, "void_layer_norm_grad")
         return dx, dw, db, None
