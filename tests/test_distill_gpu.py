@@ -309,6 +309,22 @@ def test_forward_mode_and_second_derivatives_are_refused(gpu):
         g.sum().backward()
 
 
+@gpu_only
+def test_offsets_past_31_bits(gpu):
+    V, k = 131072, 20
+    R = (1 << 31) // V + 3
+    s, t, idx = inputs(gpu, 16, V, k, torch.bfloat16)
+    s, t, idx = (a.repeat(-(-R // 16), 1)[:R].contiguous() for a in (s, t, idx))
+    ends = s[-20:], t[-20:], idx[-20:]
+    want, grad, _, bound, egrad = reference(*ends, 2.0)
+    near(void_amd.distillation_loss(s, t, idx, temperature=2.0, reduction="none")[-20:], want, bound, "row losses")
+    by = egrad + U[s.dtype] * (grad.abs() + egrad) + 2.0 ** -22 * grad.abs()
+    near(void_amd.distillation_loss_and_grad(s, t, idx, 2.0, "sum")[1][-20:], grad, by, "gradient in one call")
+    s.requires_grad_()
+    ds, = torch.autograd.grad(void_amd.distillation_loss(s, t, idx, 2.0, "sum"), s)
+    near(ds[-20:], grad, by, "gradient")
+
+
 def test_refusals():
     s, t, i = torch.randn(2, 50), torch.randn(2, 4), torch.zeros(2, 4, dtype=torch.int64)
     for call in (void_amd.distillation_loss, void_amd.distillation_loss_and_grad):
@@ -323,6 +339,9 @@ def test_refusals():
         for bad in ((s, t[:, :3], i), (s, t[:1], i[:1]), (s[0], t, i), (s, t[0, 0], i[0, 0])):
             with pytest.raises(ValueError):
                 call(*bad)
+        for V in (1 << 30, (1 << 32) + 4):  # columns that 31 or 32 bits do not hold
+            with pytest.raises(ValueError, match="long"):
+                call(torch.zeros(1).expand(2, V), t, i)
         with pytest.raises(ValueError, match="1024"):
             call(s, torch.zeros(2, 1025), torch.zeros(2, 1025, dtype=torch.int64))
         for T in (0.0, -1.0, float("nan"), float("inf")):
@@ -341,7 +360,7 @@ def test_abi_refusals():
     at = 1 << 20  # a non-null, aligned address that is never read: every call below is refused
     base = dict(logits=at, ld=50, teacher=at, ldt=4, index=at, ldi=4, rows=2, vocab=50, k=4, dtype=0, teacher_dtype=0,
                 index_bytes=8, temperature=1.0)
-    for bad, code in ((dict(rows=-1), -1), (dict(k=1025), -2), (dict(dtype=3), -2), (dict(index_bytes=2), -2),
+    for bad, code in ((dict(rows=-1), -1), (dict(k=1025), -2), (dict(vocab=1 << 30, ld=1 << 30), -2), (dict(dtype=3), -2), (dict(index_bytes=2), -2),
                       (dict(temperature=0.0), -1), (dict(logits=None), -1), (dict(index=at + 4), -1), (dict(ld=-1), -1)):
         a = _lib.DistillArgs(**{**base, **bad})
         assert lib.void_distill_loss(ctypes.byref(a), at, at, at, None) == code, bad

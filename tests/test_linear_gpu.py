@@ -302,6 +302,35 @@ def test_forward_mode_and_second_derivatives_are_refused(gpu):
         g.sum().backward()
 
 
+@gpu_only
+def test_offsets_past_31_bits(gpu):
+    # A long X, whose gradient and whose product with dZ pass them; a long Y, slope and residual.
+    x, w, b, _, _ = inputs(gpu, 128, 64, 4096, torch.bfloat16)
+    M = (1 << 31) // 4096 + 40
+    x = x.repeat(-(-M // 128), 1)[:M].requires_grad_()
+    w.requires_grad_()
+    y = void_amd.fused_linear(x, w, b)
+    dy = torch.zeros_like(y)
+    dy[-70:] = torch.randn(70, 64, device=gpu).to(y.dtype)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    tail = x.detach()[-70:], w.detach()
+    want, bound = reference(*tail, b, None, dy[-70:], "none")
+    close(y.detach()[-70:], want[0], bound[0], "y")
+    close(dx[-70:], want[1], bound[1], "dx")
+    close(dw, want[2], bound[2], "dw")  # rows of zeros add nothing
+    assert not dx[:-70].any()
+    del x, y, dy, dx, dw
+    x, w, b, _, _ = inputs(gpu, 128, 8192, 64, torch.bfloat16)
+    M = (1 << 31) // 8192 + 40
+    x = x.repeat(-(-M // 128), 1)[:M].requires_grad_()
+    r = torch.randn(64, 8192, device=gpu, dtype=torch.bfloat16).repeat(-(-M // 64), 1)[:M]
+    y = void_amd.fused_linear(x, w, b, "silu", r)
+    dx, = torch.autograd.grad(y, x, r)
+    want, bound = reference(x.detach()[-70:], w, b, r[-70:], r[-70:], "silu")
+    close(y.detach()[-70:], want[0], bound[0], "y")
+    close(dx[-70:], want[1], bound[1], "dx")
+
+
 def test_refusals():
     x, w = torch.randn(2, 8), torch.randn(4, 8)
     f = void_amd.fused_linear

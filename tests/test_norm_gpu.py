@@ -234,6 +234,20 @@ def test_forward_mode_and_second_derivatives_are_refused(gpu):
         g.sum().backward()
 
 
+@gpu_only
+def test_offsets_past_31_bits(gpu):
+    R, C = (1 << 31) // 8192 + 5, 8192
+    x = torch.randn(64, C, device=gpu, dtype=torch.bfloat16).repeat(-(-R // 64), 1)[:R]
+    w, b = torch.randn(2, C, device=gpu, dtype=torch.bfloat16)
+    x.requires_grad_()
+    y = void_amd.layer_norm(x, w, b)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    ends = [t.detach()[-70:] for t in (x, y, dx)]
+    (ry, rx, _, _), (ey, ex, _, _) = reference(ends[0], w, b, ends[0])
+    close(ends[1], ry, ey, "y")
+    close(ends[2], rx, ex, "dx")
+
+
 def test_refusals():
     x = torch.randn(2, 8)
     with pytest.raises(RuntimeError, match="GPU"):
@@ -248,6 +262,9 @@ def test_refusals():
         void_amd.layer_norm(x, None, torch.ones(1))
     with pytest.raises(ValueError):
         void_amd.layer_norm(torch.tensor(1.0))
+    for C in (1 << 30, (1 << 32) + 4):  # columns that 31 or 32 bits do not hold
+        with pytest.raises(ValueError, match="long"):
+            void_amd.layer_norm(torch.zeros(1).expand(C))
 
 
 def test_abi_refusals():
@@ -256,7 +273,7 @@ def test_abi_refusals():
     one = 1 << 20  # a non-null, aligned address that is never read: every call below is refused
     ok = dict(x=one, ldx=8, w=None, b=None, pd=0, rows=2, cols=8, eps=1e-5, dt=0, y=one, ldy=8, stats=None, stream=None)
     for bad, code in ((dict(x=None), -1), (dict(y=None), -1), (dict(rows=-1), -1), (dict(ldy=7), -1), (dict(x=one + 2), -1),
-                      (dict(dt=3), -2), (dict(pd=1), -2), (dict(stats=one + 4), -1)):
+                      (dict(dt=3), -2), (dict(cols=1 << 30, ldx=1 << 30, ldy=1 << 30), -2), (dict(pd=1), -2), (dict(stats=one + 4), -1)):
         assert lib.void_layer_norm(*{**ok, **bad}.values()) == code, bad
     args = [one, 8, one, 8, None, 0, one, 2, 8, 0, one, 8, one, one, None, 0, None]
     assert lib.void_layer_norm_grad(*args) == -4  # no workspace

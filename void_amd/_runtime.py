@@ -59,6 +59,8 @@ def vector_f32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t.reshape(-1).to(device=device, dtype=torch.float32).contiguous()
 
 
+MAX_ROW = 1 << 30  # values of a row that the row kernels take stay below (their columns are 31-bit)
+
 FLOAT_CODES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 

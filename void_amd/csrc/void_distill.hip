@@ -736,6 +736,7 @@ int launched() {
 int check(const void_distill_args* d) {
   if (!d) return void_internal_fail(VOID_ERR_ARG, "null arguments");
   if (d->rows < 0 || d->vocab < 0 || d->k < 0) return void_internal_fail(VOID_ERR_ARG, "negative size");
+  if (d->vocab > INT_MAX / 2) return void_internal_fail(VOID_ERR_UNSUPPORTED, "vocabularies are limited to 2^30 values");
   if (d->k > kMaxEntries) return void_internal_fail(VOID_ERR_UNSUPPORTED, "too many teacher entries a row");
   auto type = [](int32_t t) { return t == VOID_DT_F32 || t == VOID_DT_BF16 || t == VOID_DT_F16; };
   if (!type(d->dtype) || !type(d->teacher_dtype))

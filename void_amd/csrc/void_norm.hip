@@ -434,6 +434,8 @@ void backward(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const 
 
 int check_rows(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype) {
   if (rows < 0 || cols < 0) return void_internal_fail(VOID_ERR_ARG, "negative size");
+  // A piece's end past the row's must not pass 31 bits.
+  if (cols > INT_MAX / 2) return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are limited to 2^30 values");
   if (dtype != VOID_DT_F32 && dtype != VOID_DT_BF16 && dtype != VOID_DT_F16)
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "values are fp32, bf16 or fp16");
   if (param_dtype != dtype && param_dtype != VOID_DT_F32)

@@ -37,6 +37,8 @@ def _checked(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, t
     if teacher.shape != index.shape or teacher.dim() == 0 or teacher.shape[:-1] != logits.shape[:-1]:
         raise ValueError(f"logits {list(logits.shape)} need teacher logits and indices [..., k] of the same rows, got "
                          f"{list(teacher.shape)} and {list(index.shape)}")
+    if logits.shape[-1] >= _runtime.MAX_ROW:
+        raise ValueError(f"a vocabulary of {logits.shape[-1]} values is too long")
     if teacher.shape[-1] > MAX_ENTRIES:
         raise ValueError(f"at most {MAX_ENTRIES} teacher entries a row, got {teacher.shape[-1]}")
     if index.dtype not in _INDEX_BYTES:

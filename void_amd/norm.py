@@ -90,6 +90,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise ValueError("layer_norm needs at least one axis")
     _runtime.float_code(x, "x")
     C = x.shape[-1]
+    if C >= _runtime.MAX_ROW:
+        raise ValueError(f"rows of {C} values are too long")
     for p, what in ((weight, "weight"), (bias, "bias")):
         if p is None:
             continue
