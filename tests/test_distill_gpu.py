@@ -310,6 +310,18 @@ def test_forward_mode_and_second_derivatives_are_refused(gpu):
 
 
 @gpu_only
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,V", [(5, 7), (600, 513), (600, 2051), (520, 9001), (513, 33001), (3, 20003), (18, 20003)])
+@pytest.mark.parametrize("shift,gap", [(1, 1), (1, 2), (2, 3)])
+def test_rows_between_dwords(gpu, dtype, R, V, shift, gap):
+    # What lies beside the rows is never seen.
+    s, t, idx = inputs(gpu, R, V, 5, dtype, seed=V, ragged=True)
+    buf = torch.full((R * (V + gap) + 8,), float("inf"), device=gpu, dtype=dtype)
+    rows = buf[shift:shift + R * (V + gap)].view(R, V + gap)[:, :V].copy_(s)
+    check(rows, t, idx, 2.0)
+
+
+@gpu_only
 def test_offsets_past_31_bits(gpu):
     V, k = 131072, 20
     R = (1 << 31) // V + 3

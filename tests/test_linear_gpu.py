@@ -303,6 +303,22 @@ def test_forward_mode_and_second_derivatives_are_refused(gpu):
 
 
 @gpu_only
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 5), (1, 9001, 131), (7, 100, 1001), (30, 33, 515), (64, 8193, 257), (50, 40, 4097)])
+@pytest.mark.parametrize("shift,gap", [(1, 0), (1, 1), (2, 3)])
+def test_rows_between_dwords(gpu, dtype, M, N, K, shift, gap):
+    # What lies beside the rows is never seen.
+    x, w, b, r, dy = inputs(gpu, M, N, K, dtype, M + N + K)
+
+    def spread(t):
+        rows, cols = t.shape
+        buf = torch.full((rows * (cols + gap) + 8,), float("nan"), device=gpu, dtype=dtype)
+        return buf[shift:shift + rows * (cols + gap)].view(rows, cols + gap)[:, :cols].copy_(t)
+    check(spread(x), spread(w), b, spread(r), spread(dy), "silu")
+    check(x, spread(w), b, None, spread(dy), "gelu")
+
+
+@gpu_only
 def test_offsets_past_31_bits(gpu):
     # A long X, whose gradient and whose product with dZ pass them; a long Y, slope and residual.
     x, w, b, _, _ = inputs(gpu, 128, 64, 4096, torch.bfloat16)

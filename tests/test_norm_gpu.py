@@ -235,6 +235,23 @@ def test_forward_mode_and_second_derivatives_are_refused(gpu):
 
 
 @gpu_only
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C", [5, 63, 257, 1500, 4097, 16383, 16391])
+@pytest.mark.parametrize("shift,gap", [(0, 1), (1, 0), (1, 1), (3, 2)])
+def test_rows_between_dwords(gpu, dtype, C, shift, gap):
+    # What lies beside the rows is never seen.
+    x, w, b, dy = inputs(gpu, dtype, 6, C, C + shift)
+
+    def spread(t, at):
+        pitch = C + gap
+        buf = torch.full((6 * pitch + 8,), float("nan"), device=gpu, dtype=dtype)
+        return buf[at:at + 6 * pitch].view(6, pitch)[:, :C].copy_(t)
+    check(spread(x, shift), w, b, spread(dy, shift))
+    check(spread(x, shift), w, b, dy)
+    check(x, w, b, spread(dy, 1))
+
+
+@gpu_only
 def test_offsets_past_31_bits(gpu):
     R, C = (1 << 31) // 8192 + 5, 8192
     x = torch.randn(64, C, device=gpu, dtype=torch.bfloat16).repeat(-(-R // 64), 1)[:R]

@@ -247,10 +247,9 @@ __device__ __forceinline__ Part join(Part x, Part y, float c) {
 
 // (m, z) of a slice, for all T threads.  Each thread keeps its own largest logit and
 // rescales its sum when a batch of kAhead pieces raises it.
-template <class E, int T>
+template <class E, int T, bool ODD>
 __device__ __forceinline__ Part slice_part(const Args& a, const E* s, const Slice<E>& sl, Areas& red) {
   constexpr int N = Piece<E>::n, kAhead = 4;
-  typedef typename Piece<E>::any Any;
   typedef typename Piece<E>::fvec F;
   float m = kLowest, z = 0.f;
   if (threadIdx.x < sl.rest) {
@@ -259,17 +258,17 @@ __device__ __forceinline__ Part slice_part(const Args& a, const E* s, const Slic
     z = pow2((x - m) * a.c);
   }
   for (uint32_t q = sl.first + threadIdx.x; q < sl.last; q += kAhead * T) {
-    typename Piece<E>::vec v[kAhead];
+    Loaded<E, ODD> v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      v[u] = (E)-INFINITY;
-      if (q + u * T < sl.last) v[u] = *reinterpret_cast<const Any*>(s + (int64_t)(q + u * T) * N);
+      v[u].lowest();
+      if (q + u * T < sl.last) v[u].whole(s + (int64_t)(q + u * T) * N);
     }
     float top = m;
     F f[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      f[u] = __builtin_convertvector(v[u], F);
+      f[u] = __builtin_convertvector(v[u].take(s), F);
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, f[u][e]);
     }
@@ -336,7 +335,7 @@ __device__ __forceinline__ int take_entries(const Args& a, int64_t row, const E*
 // LOSS (S = 1) the row's loss too.  Clears `arrived` (unless null).  Bound by reading the logits: 4096 x 32768 bf16
 // 52 us, 5.2 TB/s; 730 x 50021 fp32 with a quarter of the rows without entries 24 us,
 // 4.5 TB/s.
-template <class E, int T, bool LOSS>
+template <class E, int T, bool LOSS, bool ODD>
 __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t units, float2* __restrict__ parts,
                                                           int32_t* __restrict__ used, float* __restrict__ loss,
                                                           int32_t* __restrict__ arrived) {
@@ -360,7 +359,7 @@ __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t
       flags = get_flags<T>(flags, red);
     }
     Part p{0.f, 1.f};
-    if (flags & kSome) p = slice_part<E, T>(a, s, Slice<E>(a.vocab, S, sl), red);
+    if (flags & kSome) p = slice_part<E, T, ODD>(a, s, Slice<E>(a.vocab, S, sl), red);
     if (threadIdx.x < 64) {
       float l = 0.f;
       if constexpr (LOSS)
@@ -433,7 +432,7 @@ __device__ __forceinline__ void add_row_loss(const Args& a, int64_t row, float l
 // 730 x 50021 fp32 with a quarter of the rows without entries 58 us, 4.4 TB/s.  What
 // the entries need of the teacher is made while the logits come (300 x 131072 bf16,
 // loss and gradient: 50.4 us, and 54.4 at the end).
-template <class E, int T>
+template <class E, int T, bool ODD>
 __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const float2* __restrict__ parts, int G,
                                                          int64_t units, const float* __restrict__ g, int64_t gstep,
                                                          const float* __restrict__ factor, float scale,
@@ -442,7 +441,6 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
                                                          float* __restrict__ total, int32_t* __restrict__ arrived) {
   constexpr int N = Piece<E>::n, kAhead = 4;
   typedef typename Piece<E>::vec V;
-  typedef typename Piece<E>::any Any;
   typedef typename Piece<E>::fvec F;
   __shared__ Areas red;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -464,11 +462,11 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
       continue;
     }
     const float gs = (g ? g[row * gstep] * scale : scale) * a.temperature;
-    V v[kAhead];
+    Loaded<E, ODD> v[kAhead];
     auto load = [&](uint32_t q) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
-        if (q + i * T < sl.last) v[i] = *reinterpret_cast<const Any*>(s + (int64_t)(q + i * T) * N);
+        if (q + i * T < sl.last) v[i].whole(s + (int64_t)(q + i * T) * N);
     };
     uint32_t q = sl.first + threadIdx.x;
     load(q);
@@ -480,7 +478,7 @@ __global__ __launch_bounds__(T) void distill_grad_kernel(Args a, int S, const fl
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (q + i * T < sl.last) {
-          F o = __builtin_convertvector(v[i], F);
+          F o = __builtin_convertvector(v[i].take(s), F);
 #pragma unroll
           for (int e = 0; e < N; ++e) o[e] = pow2((o[e] - st.m) * a.c) * f;
           stream_out(ds + (int64_t)(q + i * T) * N, __builtin_convertvector(o, V));
@@ -529,13 +527,12 @@ __global__ __launch_bounds__(1024) void distill_count_kernel(Args a, int32_t* __
 // load and store.  Bound by the memory: 8192 x 65536 bf16 466 us, 4.6 TB/s of one read
 // and one write; x 131072 967 us, 4.45, with a quarter of the rows without entries
 // 820 to 870 us, 4.3 to 4.6 (a copy of 2 GiB: 4.94).
-template <class E, int T, int NV>
+template <class E, int T, int NV, bool ODD>
 __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale, const int32_t* __restrict__ counts,
                                                             int n_counts, E* __restrict__ grad, int64_t ldg,
                                                             float* __restrict__ loss, int32_t* __restrict__ used) {
   constexpr int N = Piece<E>::n, kAhead = 2;
   typedef typename Piece<E>::vec V;
-  typedef typename Piece<E>::any Any;
   typedef typename Piece<E>::fvec F;
   __shared__ Areas red;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -561,29 +558,33 @@ __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale,
 #pragma unroll
       for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
     };
-    each_of(
-        [&](auto i) {
-          const uint32_t q = (uint32_t)i.value * T + threadIdx.x;
-          v[i.value] = (E)-INFINITY;
-          if (q < whole) v[i.value] = *reinterpret_cast<const Any*>(s + (int64_t)q * N);
-        },
-        pieces_each);
+    {
+      Loaded<E, ODD> in[NV];
+      each_of(
+          [&](auto i) {
+            const uint32_t q = (uint32_t)i.value * T + threadIdx.x;
+            in[i.value].lowest();
+            if (q < whole) in[i.value].whole(s + (int64_t)q * N);
+          },
+          pieces_each);
+      each_of([&](auto i) { v[i.value] = in[i.value].take(s); }, pieces_each);
+    }
     const float tail = threadIdx.x < rest ? (float)s[(int64_t)whole * N + threadIdx.x] : -INFINITY;
     // A thread's own largest logit first: what lies behind the registers, rescaling
     // its sum as it rises, then the registers.
     float m = kLowest, z = 0.f;
 #pragma unroll 1
     for (uint32_t q = NV * T + threadIdx.x; q < whole; q += kAhead * T) {
-      V w[kAhead];
+      Loaded<E, ODD> w[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        w[u] = (E)-INFINITY;
-        if (q + u * T < whole) w[u] = *reinterpret_cast<const Any*>(s + (int64_t)(q + u * T) * N);
+        w[u].lowest();
+        if (q + u * T < whole) w[u].whole(s + (int64_t)(q + u * T) * N);
       }
       float top = m;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const F f = __builtin_convertvector(w[u], F);
+        const F f = __builtin_convertvector(w[u].take(s), F);
 #pragma unroll
         for (int e = 0; e < N; ++e) top = fmaxf(top, f[e]);
       }
@@ -591,7 +592,7 @@ __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale,
       m = top;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const F f = __builtin_convertvector(w[u], F);
+        const F f = __builtin_convertvector(w[u].take(s), F);
 #pragma unroll
         for (int e = 0; e < N; ++e) z += pow2((f[e] - m) * a.c);
       }
@@ -636,14 +637,14 @@ __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale,
         pieces_each);
 #pragma unroll 1
     for (uint32_t q = NV * T + threadIdx.x; q < whole; q += kAhead * T) {
-      V w[kAhead];
+      Loaded<E, ODD> w[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (q + u * T < whole) w[u] = *reinterpret_cast<const Any*>(s + (int64_t)(q + u * T) * N);
+        if (q + u * T < whole) w[u].whole(s + (int64_t)(q + u * T) * N);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
         if (q + u * T < whole) {
-          F o = __builtin_convertvector(w[u], F);
+          F o = __builtin_convertvector(w[u].take(s), F);
 #pragma unroll
           for (int e = 0; e < N; ++e) o[e] = pow2((o[e] - m) * a.c) * f0;
           stream_out(ds + (int64_t)(q + u * T) * N, __builtin_convertvector(o, V));
@@ -760,22 +761,23 @@ Args args_of(const void_distill_args* d) {
 }
 
 template <class E>
-void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, int32_t* arrived,
-           hipStream_t stream) {
+void parts(const Args& a, int S, float2* part, int32_t* used, float* loss, int32_t* arrived, hipStream_t stream) {
   const int64_t units = a.rows * S;
   by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, S > 1, [&](auto t) {
-    constexpr int T = decltype(t)::value;
-    const dim3 grid((unsigned)std::min(units, kMaxGrid));
-    if (S == 1 && loss)
-      hipLaunchKernelGGL((distill_parts_kernel<E, T, true>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part,
-                         used, loss, arrived);
-    else
-      hipLaunchKernelGGL((distill_parts_kernel<E, T, false>), grid, dim3(T), entries_bytes(a.k), stream, a, S, units, part,
-                         used, loss, arrived);
+    by_parity<E>(a.logits, a.ld, nullptr, 0, a.rows, [&](auto odd) {
+      constexpr int T = decltype(t)::value;
+      constexpr bool ODD = decltype(odd)::value;
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, kMaxGrid)), dim3(T), entries_bytes(a.k), stream, a, S,
+                           units, part, used, loss, arrived);
+      };
+      if (S == 1 && loss) go(distill_parts_kernel<E, T, true, ODD>);
+      else go(distill_parts_kernel<E, T, false, ODD>);
+    });
   });
   if (S > 1 && loss)
-    hipLaunchKernelGGL(distill_loss_kernel<E>, dim3((unsigned)std::min(a.rows, kMaxGrid)), dim3(64), entries_bytes(a.k), stream, a, S,
-                       part, loss);
+    hipLaunchKernelGGL(distill_loss_kernel<E>, dim3((unsigned)std::min(a.rows, kMaxGrid)), dim3(64), entries_bytes(a.k),
+                       stream, a, S, part, loss);
 }
 
 template <class E>
@@ -784,9 +786,12 @@ void gradient(const Args& a, int S, const float2* part, const float* g, int64_t 
               hipStream_t stream) {
   const int64_t units = a.rows * S;
   by_length(((int64_t)a.vocab / S + Piece<E>::n - 1) / Piece<E>::n, S > 1, [&](auto t) {
-    constexpr int T = decltype(t)::value;
-    hipLaunchKernelGGL((distill_grad_kernel<E, T>), dim3((unsigned)std::min(units, kMaxGrid)), dim3(T), entries_bytes(a.k), stream, a, S,
-                       part, S, units, g, gstep, factor, scale, counts, n_counts, static_cast<E*>(grad), ldg, loss, total, arrived);
+    by_parity<E>(a.logits, a.ld, nullptr, 0, a.rows, [&](auto odd) {
+      constexpr int T = decltype(t)::value;
+      hipLaunchKernelGGL((distill_grad_kernel<E, T, decltype(odd)::value>), dim3((unsigned)std::min(units, kMaxGrid)),
+                         dim3(T), entries_bytes(a.k), stream, a, S, part, S, units, g, gstep, factor, scale, counts,
+                         n_counts, static_cast<E*>(grad), ldg, loss, total, arrived);
+    });
   });
 }
 
@@ -892,9 +897,14 @@ int void_distill_step(const void_distill_args* d, int32_t mean, float grad_scale
       const int n = count_grid(d->rows);
       if (mean) hipLaunchKernelGGL(distill_count_kernel, dim3(n), dim3(1024), 0, stream, a, counts);
       by_row<E>(d->vocab, [&](auto t, auto nv) {
-        constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
-        hipLaunchKernelGGL((distill_step_kernel<E, T, NV>), dim3((unsigned)std::min(d->rows, kMaxGrid)), dim3(T), entries_bytes(a.k), stream, a, grad_scale, mean ? counts : nullptr, n,
-                           static_cast<E*>(grad), ldg, row_loss, used);
+        by_parity<E>(d->logits, d->ld, nullptr, 0, d->rows, [&](auto odd) {
+          constexpr int T = decltype(t)::value;
+          constexpr int NV = decltype(nv)::value;
+          constexpr bool ODD = decltype(odd)::value;
+          hipLaunchKernelGGL((distill_step_kernel<E, T, NV, ODD>), dim3((unsigned)std::min(d->rows, kMaxGrid)), dim3(T),
+                             entries_bytes(a.k), stream, a, grad_scale, mean ? counts : nullptr, n,
+                             static_cast<E*>(grad), ldg, row_loss, used);
+        });
       });
       sum();
       return;

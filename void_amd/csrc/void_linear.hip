@@ -665,11 +665,11 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // rows of W, each wave a share of K straight from memory into fragments (no LDS:
 // nothing of W is used twice), any alignment; the waves' sums are added in order.
 // One token x 14336 x 4096 bf16 25.6 us, 4.6 TB/s.
-template <class E, int MT, int NW>
+template <class E, int MT, int NW, bool ODD>
 __global__ __launch_bounds__(64 * NW) void few_kernel(const E* __restrict__ x, int64_t ldx, const E* __restrict__ w,
                                                       int64_t ldw, int M, int64_t N, int K, Epilogue epi) {
   constexpr int kPer = Piece<E>::n, kStep = 4 * kPer;  // 64 bytes of a row: a chunk each for 4 lanes
-  constexpr int kAhead = 4;
+  constexpr int kAhead = ODD && MT == 4 ? 2 : 4;  // as much as fits the registers
   typedef typename Piece<E>::vec V;
   __shared__ v4f sum[NW][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -694,22 +694,23 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(const E* __restrict__ x, i
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(xv, wv, c, 0, 0, 0);
     }
   };
-  typedef typename Piece<E>::any Any;
   // Whole steps: the waves take groups of kAhead in turn.
   const int steps = K / kStep, groups = steps / kAhead;
   for (int q = wave; q < groups; q += NW) {
     const int k0 = q * kAhead * kStep;
-    V wv[kAhead], xv[kAhead][MT];
+    Loaded<E, ODD> wv[kAhead], xv[kAhead][MT];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      wv[u] = *reinterpret_cast<const Any*>(wr + k0 + u * kStep);
+      wv[u].whole(wr + k0 + u * kStep);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) xv[u][t] = *reinterpret_cast<const Any*>(xr[t] + k0 + u * kStep);
+      for (int t = 0; t < MT; ++t) xv[u][t].whole(xr[t] + k0 + u * kStep);
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
+    for (int u = 0; u < kAhead; ++u) {
+      const V w4 = wv[u].take(wr);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t] = multiply(wv[u], xv[u][t], acc[t]);
+      for (int t = 0; t < MT; ++t) acc[t] = multiply(w4, xv[u][t].take(xr[t]), acc[t]);
+    }
   }
   // The rest, a step a wave; past K both operands are zero.
   for (int q = groups * kAhead + wave; q * kStep < K; q += NW) {
@@ -744,7 +745,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(const E* __restrict__ x, i
 // this workgroup's column sums in part[blockIdx.y][N] (unless part is null).  64
 // pieces of columns, 4 rows at a time.  Bound by the memory: 8192 x 14336 bf16 154 us,
 // 4.6 TB/s of dy, the slope and dz.
-template <class E>
+template <class E, bool ODD>
 __global__ __launch_bounds__(256) void slope_kernel(const E* __restrict__ dy, int64_t lddy,
                                                     const typename Slope<E>::type* __restrict__ slope, int64_t M, int N,
                                                     E* __restrict__ dz, int64_t ldz, float* __restrict__ part) {
@@ -753,7 +754,6 @@ __global__ __launch_bounds__(256) void slope_kernel(const E* __restrict__ dy, in
   typedef typename Piece<E>::fvec F;
   typedef typename Slope<E>::type S;
   typedef S SV __attribute__((ext_vector_type(16 / sizeof(E))));
-  typedef SV SAny __attribute__((aligned(sizeof(S))));
   __shared__ float sum[4][64 * n];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c64 = ((int64_t)blockIdx.x * 64 + lane) * n;
@@ -761,17 +761,17 @@ __global__ __launch_bounds__(256) void slope_kernel(const E* __restrict__ dy, in
   if (c64 < N) {
     const int c = (int)c64;
     for (int64_t row = (int64_t)blockIdx.y * 4 + wave; row < M; row += (int64_t)gridDim.y * 4) {
-      F f = __builtin_convertvector(load_piece(dy + row * lddy, c, N), F);
+      const E* dr = dy + row * lddy;
+      const S* sr = slope + row * N;
+      Loaded<E, ODD> v;
+      Loaded<S, ODD> sv;
+      v.load(dr, c, N);
+      if (slope) sv.load(sr, c, N);
+      F f = __builtin_convertvector(v.take(dr, c, N), F);
       if (slope) {
-        const S* sr = slope + row * N + c;
-        if (c + n <= N) {
-          const SV v = *reinterpret_cast<const SAny*>(sr);
+        const SV s4 = sv.take(sr, c, N);
 #pragma unroll
-          for (int e = 0; e < n; ++e) f[e] *= Slope<E>::unpack(v[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < n; ++e) f[e] = c + e < N ? f[e] * Slope<E>::unpack(sr[e]) : 0.f;
-        }
+        for (int e = 0; e < n; ++e) f[e] = c + e < N ? f[e] * Slope<E>::unpack(s4[e]) : 0.f;
         if (dz) *reinterpret_cast<V*>(dz + row * ldz + c) = __builtin_convertvector(f, V);
       }
       s += f;
@@ -890,9 +890,11 @@ template <class E>
 void few(const void_linear_args* d, const Epilogue& epi, hipStream_t stream) {
   auto go = [&](auto mt, auto nw) {
     constexpr int MT = decltype(mt)::value, NW = decltype(nw)::value;
-    hipLaunchKernelGGL((few_kernel<E, MT, NW>), dim3((unsigned)((d->N + 15) / 16)), dim3(64 * NW), 0, stream,
-                       static_cast<const E*>(d->x), d->ldx, static_cast<const E*>(d->w), d->ldw, (int)d->M, d->N,
-                       (int)d->K, epi);
+    by_parity<E>(d->x, d->ldx, d->w, d->ldw, std::max(d->M, d->N), [&](auto odd) {
+      hipLaunchKernelGGL((few_kernel<E, MT, NW, decltype(odd)::value>), dim3((unsigned)((d->N + 15) / 16)), dim3(64 * NW),
+                         0, stream, static_cast<const E*>(d->x), d->ldx, static_cast<const E*>(d->w), d->ldw, (int)d->M,
+                         d->N, (int)d->K, epi);
+    });
   };
   auto waves = [&](auto mt) {
     if (d->N >= 8192) go(mt, std::integral_constant<int, 4>{});
@@ -1075,9 +1077,12 @@ int void_linear_grad_z(const void* dy, int64_t lddy, const void* slope, int64_t 
   by_type(dtype, [&](auto e) {
     using E = decltype(e);
     if (M)
-      hipLaunchKernelGGL(slope_kernel<E>, dim3((unsigned)((N * esz + 1023) / 1024), gy), dim3(256), 0, stream,
-                         static_cast<const E*>(dy), lddy, static_cast<const typename Slope<E>::type*>(slope), M, (int)N,
-                         static_cast<E*>(dz), ldz, db ? static_cast<float*>(workspace) : nullptr);
+      by_parity<E>(dy, lddy, slope, slope ? N : 0, M, [&](auto odd) {
+        hipLaunchKernelGGL((slope_kernel<E, decltype(odd)::value>), dim3((unsigned)((N * esz + 1023) / 1024), gy),
+                           dim3(256), 0, stream, static_cast<const E*>(dy), lddy,
+                           static_cast<const typename Slope<E>::type*>(slope), M, (int)N, static_cast<E*>(dz), ldz,
+                           db ? static_cast<float*>(workspace) : nullptr);
+      });
     if (db) {
       const dim3 grid((unsigned)((N + 63) / 64));
       if (bias_dtype == VOID_DT_F32)

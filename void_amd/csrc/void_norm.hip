@@ -36,7 +36,7 @@ constexpr int block_of(int T) { return T < 256 ? 256 : T; }
 // One read of x, one write of y.  16384 x 8192 bf16 91 us, 5.9 TB/s; 2048 x 4096 bf16
 // 10.6 us, in the caches; 5003 x 3001 fp32 27 us, 4.4 TB/s; one row of 4096 3.1 us, which
 // is the launch and two sums.
-template <class E, class W, int T, int NV>
+template <class E, class W, int T, int NV, bool ODD>
 __global__ __launch_bounds__(block_of(T)) void norm_kernel(const E* __restrict__ x, int64_t ldx,
                                                            const W* __restrict__ weight, const W* __restrict__ bias,
                                                            int64_t rows, int cols, float eps, E* __restrict__ y,
@@ -50,10 +50,10 @@ __global__ __launch_bounds__(block_of(T)) void norm_kernel(const E* __restrict__
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T;
   const float inv = 1.f / (float)cols;
-  V v[NV];
+  Loaded<E, ODD> v[NV];
   if (row < rows)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = load_piece(x + row * ldx, (i * T + t) * N, cols);
+    for (int i = 0; i < NV; ++i) v[i].load(x + row * ldx, (i * T + t) * N, cols);
   float w[NV][N], b[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -63,10 +63,10 @@ __global__ __launch_bounds__(block_of(T)) void norm_kernel(const E* __restrict__
   for (; row < rows; row += step) {
     F f[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = __builtin_convertvector(v[i], F);
+    for (int i = 0; i < NV; ++i) f[i] = __builtin_convertvector(v[i].take(x + row * ldx, (i * T + t) * N, cols), F);
     if (row + step < rows)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] = load_piece(x + (row + step) * ldx, (i * T + t) * N, cols);
+      for (int i = 0; i < NV; ++i) v[i].load(x + (row + step) * ldx, (i * T + t) * N, cols);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const E* __restrict__ x
 // `part` is null) in part[2 blockIdx.x] and part[2 blockIdx.x + 1], rows of
 // `cols` floats.  One read of x and dy, one write of dx: 16384 x 8192 bf16 156 us,
 // 5.1 TB/s; 2048 x 4096 bf16 14.5 us; 5003 x 3001 fp32 44 us, 4.1 TB/s.
-template <class E, class W, int T, int NV>
+template <class E, class W, int T, int NV, bool ODD>
 __global__ __launch_bounds__(block_of(T)) void norm_grad_kernel(
     const E* __restrict__ dy, int64_t lddy, const E* __restrict__ x, int64_t ldx, const W* __restrict__ weight,
     const float2* __restrict__ stats, int64_t rows, int cols, E* __restrict__ dx, int64_t lddx,
@@ -159,14 +159,14 @@ __global__ __launch_bounds__(block_of(T)) void norm_grad_kernel(
   const float inv = 1.f / (float)cols;
   // 1024 threads have 128 registers each: no room for the next row's pieces.
   constexpr bool kAhead = T < 1024;
-  V vx[NV], vg[NV];
+  Loaded<E, ODD> vx[NV], vg[NV];
   float2 st = {};
   auto fetch = [&](int64_t r) {
     st = stats[r];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      vx[i] = load_piece(x + r * ldx, (i * T + t) * N, cols);
-      vg[i] = load_piece(dy + r * lddy, (i * T + t) * N, cols);
+      vx[i].load(x + r * ldx, (i * T + t) * N, cols);
+      vg[i].load(dy + r * lddy, (i * T + t) * N, cols);
     }
   };
   if (kAhead && row < rows) fetch(row);
@@ -184,8 +184,8 @@ __global__ __launch_bounds__(block_of(T)) void norm_grad_kernel(
     const float r = st.y;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      h[i] = __builtin_convertvector(vx[i], F);
-      g[i] = __builtin_convertvector(vg[i], F);
+      h[i] = __builtin_convertvector(vx[i].take(x + row * ldx, (i * T + t) * N, cols), F);
+      g[i] = __builtin_convertvector(vg[i].take(dy + row * lddy, (i * T + t) * N, cols), F);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         // Past the row's end dy is zero, so only what is stored could see h there.
@@ -400,8 +400,10 @@ void forward(const void* x, int64_t ldx, const void* w, const void* b, int64_t r
   };
   if (!by_width<E>(cols, [&](auto t, auto nv) {
         constexpr int T = decltype(t)::value, NV = decltype(nv)::value, kRows = block_of(T) / T;
-        args(norm_kernel<E, W, T, NV>, std::min<int64_t>((rows + kRows - 1) / kRows, kCus * (T > 256 ? 2 : 4)),
-             block_of(T));
+        by_parity<E>(x, ldx, x, ldx, rows, [&](auto odd) {
+          args(norm_kernel<E, W, T, NV, decltype(odd)::value>,
+               std::min<int64_t>((rows + kRows - 1) / kRows, kCus * (T > 256 ? 2 : 4)), block_of(T));
+        });
       }))
     args(norm_long_kernel<E, W>, std::min<int64_t>(rows, kCus * 2), 1024);
 }
@@ -416,8 +418,10 @@ void backward(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const 
   const int n = partials<E>(rows, cols);
   if (!by_width<E>(cols, [&](auto t, auto nv) {
         constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
-        hipLaunchKernelGGL((norm_grad_kernel<E, W, T, NV>), dim3(n), dim3(block_of(T)), 0, stream, dy, lddy, x, ldx, w,
-                           stats, rows, cols, dx, lddx, part);
+        by_parity<E>(dy, lddy, x, ldx, rows, [&](auto odd) {
+          hipLaunchKernelGGL((norm_grad_kernel<E, W, T, NV, decltype(odd)::value>), dim3(n), dim3(block_of(T)), 0,
+                             stream, dy, lddy, x, ldx, w, stats, rows, cols, dx, lddx, part);
+        });
       })) {
     if (dx)
       hipLaunchKernelGGL((norm_long_grad_kernel<E, W>), dim3((unsigned)std::min<int64_t>(rows, kCus * 2)), dim3(1024),
