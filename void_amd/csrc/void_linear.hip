@@ -826,8 +826,9 @@ struct Plan {
 // `full` a step of 128 bytes along r where a CU has one tile and, per tile, where it
 // has two; splits add a launch and their sums' traffic.  The figures are fitted to 400
 // timings of 18 bf16 and 8 fp32 products (17 to 8192 rows, 512 to 14336 columns, depths
-// of 512 to 14336; the estimates are within 15 %, the plans chosen 2 % and 0.4 % slower
-// than each product's best).
+// of 512 to 14336; the estimates are within 15 %, but for products of several rounds of
+// 256-row tiles, which the chip's power makes up to a fifth slower; the plans chosen are
+// 1 to 2 % and 0.4 % slower than each product's best).
 struct Cost {
   int tile;
   double fixed, alone, full, join, traffic;
