@@ -43,7 +43,8 @@ def _checked(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, t
         raise ValueError(f"at most {MAX_ENTRIES} teacher entries a row, got {teacher.shape[-1]}")
     if index.dtype not in _INDEX_BYTES:
         raise TypeError(f"teacher indices must be int32 or int64, got {index.dtype}")
-    code, tcode = _runtime.float_code(logits, "logits"), _runtime.float_code(teacher, "teacher logits")
+    _runtime.float_code(logits, "logits")
+    _runtime.float_code(teacher, "teacher logits")
     temperature = float(temperature)
     if not (0 < temperature < math.inf):
         raise ValueError(f"the temperature must be positive, got {temperature}")
@@ -52,9 +53,15 @@ def _checked(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, t
         if t.device != logits.device:
             raise ValueError(f"logits on {logits.device}, {what} on {t.device}")
     s, t, i = _flat(logits), _flat(teacher), _flat(index)
+    return s, t, i, _args(s, t, i, temperature)
+
+
+def _args(s: torch.Tensor, t: torch.Tensor, i: torch.Tensor, temperature: float) -> "_lib.DistillArgs":
+    """The C arguments over rows of logits, teacher logits and indices."""
     R, V = s.shape
-    return s, t, i, _lib.DistillArgs(s.data_ptr(), s.stride(0), t.data_ptr(), t.stride(0), i.data_ptr(), i.stride(0), R,
-                                     V, t.shape[1], code, tcode, _INDEX_BYTES[index.dtype], temperature)
+    return _lib.DistillArgs(s.data_ptr(), s.stride(0), t.data_ptr(), t.stride(0), i.data_ptr(), i.stride(0), R, V,
+                            t.shape[1], _runtime.FLOAT_CODES[s.dtype], _runtime.FLOAT_CODES[t.dtype],
+                            _INDEX_BYTES[i.dtype], temperature)
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
@@ -96,18 +103,20 @@ class _Distillation(Function):
         loss, parts, used = _losses(args, s.device)
         out, factor = (loss.view(logits.shape[:-1]), None) if reduction == "none" else _reduced(loss, used, reduction)
         ctx.save_for_backward(s, t, i, parts, factor)
-        ctx.args, ctx.shape = args, logits.shape
+        ctx.temperature, ctx.shape = args.temperature, logits.shape
         return out
 
     @staticmethod
     @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
+        # What a hook or a checkpoint gives back need not lie where the forward pass had it.
         s, t, i, parts, factor = ctx.saved_tensors
+        args = _args(s, t, i, ctx.temperature)
         ds = s.new_empty(ctx.shape)
         if not ds.numel():
             return ds, None, None, None, None
         g = grad.reshape(-1).to(torch.float32)
-        st = _lib.lib().void_distill_grad(ctypes.byref(ctx.args), parts.data_ptr(), g.data_ptr(),
+        st = _lib.lib().void_distill_grad(ctypes.byref(args), parts.data_ptr(), g.data_ptr(),
                                           g.stride(0) if factor is None else 0,
                                           factor.data_ptr() if factor is not None else None, ds.data_ptr(), s.shape[1],
                                           raw_stream(s.device))
