@@ -109,8 +109,9 @@ class _Distillation(Function):
     @staticmethod
     @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
-        # What a hook or a checkpoint gives back need not lie where the forward pass had it.
+        # What a hook or a checkpoint gives back need not lie where the forward pass had it, nor in its layout.
         s, t, i, parts, factor = ctx.saved_tensors
+        s, t, i, parts = _flat(s), _flat(t), _flat(i), parts.contiguous()
         args = _args(s, t, i, ctx.temperature)
         ds = s.new_empty(ctx.shape)
         if not ds.numel():

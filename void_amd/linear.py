@@ -109,7 +109,9 @@ class _FusedLinear(Function):
     @staticmethod
     @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
+        # What a hook or a checkpoint gives back need not lie in the layout that the forward pass saved.
         rows, w, slope = ctx.saved_tensors
+        slope = None if slope is None else slope.contiguous()
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         lib, (N, K) = _lib.lib(), ctx.w_shape
         M, dev, dtype = math.prod(ctx.x_shape[:-1]), grad.device, grad.dtype

@@ -53,7 +53,10 @@ class _LayerNorm(Function):
     @staticmethod
     @_runtime.first_order
     def backward(ctx: Any, grad: torch.Tensor):
+        # What a hook or a checkpoint gives back need not lie in the layout that the forward pass saved.
         rows, weight, stats = ctx.saved_tensors
+        rows, stats = _runtime.flat_rows(rows), stats.contiguous()
+        weight = None if weight is None else weight.contiguous()
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         R, C = rows.shape
         dy = _runtime.flat_rows(grad)
