@@ -149,6 +149,22 @@ def test_empty(gpu, shape):
 
 
 @gpu_only
+@pytest.mark.parametrize("shape", [(2, 3, 0), (0, 3, 5), (2, 0, 5), (2, 0, 0)])
+def test_empty_axes_of_more_dimensions(gpu, shape):
+    x = torch.empty(shape, device=gpu, requires_grad=True)
+    w, b = (torch.ones(shape[-1], device=gpu, requires_grad=True) for _ in range(2))
+    y = void_amd.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert y.shape == dx.shape == shape and not dw.any() and not db.any() and dw.shape == db.shape == (shape[-1],)
+
+
+def test_rows_of_empty_tensors():
+    from void_amd import _runtime
+    for shape, rows in (((2, 3, 0), (6, 0)), ((0, 3, 5), (0, 5)), ((2, 0, 0), (0, 0)), ((0,), (1, 0)), ((5,), (1, 5))):
+        assert _runtime.flat_rows(torch.empty(shape)).shape == rows
+
+
+@gpu_only
 @pytest.mark.parametrize("C", [50, 3000, 17000])
 def test_non_finite_rows_stay_alone(gpu, C):
     x, w, b, dy = inputs(gpu, torch.float32, 8, C)

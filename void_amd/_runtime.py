@@ -10,6 +10,7 @@ into ``libvoid_amd.so`` on the current torch stream.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import threading
 from dataclasses import dataclass, field
@@ -93,7 +94,7 @@ def first_order(backward):
 def flat_rows(t: torch.Tensor) -> torch.Tensor:
     """t as a 2-D tensor of its last axis's rows with unit column stride; a
     view wherever the strides allow one (rows of any pitch, one row repeated)."""
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    t = t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])  # -1 is ambiguous for empty rows
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 

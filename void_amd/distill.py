@@ -52,7 +52,7 @@ def _checked(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, t
     for t, what in ((teacher, "teacher logits"), (index, "teacher indices")):
         if t.device != logits.device:
             raise ValueError(f"logits on {logits.device}, {what} on {t.device}")
-    s, t, i = _flat(logits), _flat(teacher), _flat(index)
+    s, t, i = _runtime.flat_rows(logits), _runtime.flat_rows(teacher), _runtime.flat_rows(index)
     return s, t, i, _args(s, t, i, temperature)
 
 
@@ -62,10 +62,6 @@ def _args(s: torch.Tensor, t: torch.Tensor, i: torch.Tensor, temperature: float)
     return _lib.DistillArgs(s.data_ptr(), s.stride(0), t.data_ptr(), t.stride(0), i.data_ptr(), i.stride(0), R, V,
                             t.shape[1], _runtime.FLOAT_CODES[s.dtype], _runtime.FLOAT_CODES[t.dtype],
                             _INDEX_BYTES[i.dtype], temperature)
-
-
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    return _runtime.flat_rows(t) if t.numel() else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
 
 
 def _losses(args: "_lib.DistillArgs", device: torch.device):
@@ -111,7 +107,7 @@ class _Distillation(Function):
     def backward(ctx: Any, grad: torch.Tensor):
         # What a hook or a checkpoint gives back need not lie where the forward pass had it, nor in its layout.
         s, t, i, parts, factor = ctx.saved_tensors
-        s, t, i, parts = _flat(s), _flat(t), _flat(i), parts.contiguous()
+        s, t, i, parts = _runtime.flat_rows(s), _runtime.flat_rows(t), _runtime.flat_rows(i), parts.contiguous()
         args = _args(s, t, i, ctx.temperature)
         ds = s.new_empty(ctx.shape)
         if not ds.numel():
