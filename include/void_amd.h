@@ -486,8 +486,8 @@ typedef struct void_linear_args {
 
 /* Products of exact fp32 terms summed in fp32, one rounding of Y.  Up to 64 rows
  * of X (void_linear_any_alignment() is 1) take operands of any alignment; more
- * need X and W 16-byte aligned with K, ldx and ldw whole 16-byte chunks (else
- * VOID_ERR_UNSUPPORTED).  Y may be the residual's array.  No counterpart in the
+ * need X and W 16-byte aligned with K, ldx and ldw whole 16-byte chunks, and 256
+ * rows of each (or all, if fewer) within 2 GiB (else VOID_ERR_UNSUPPORTED).  Y may be the residual's array.  No counterpart in the
  * reference. */
 int32_t void_linear_any_alignment(int64_t M);
 size_t void_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype);
@@ -503,7 +503,8 @@ int void_linear_grad_z(const void* dy, int64_t lddy, const void* slope, int64_t 
                        hipStream_t stream);
 
 /* dX [M, K] = dZ [M, N] W [N, K] and dW [N, K] = dZ^T X.  dZ, W and X: 16-byte
- * aligned rows of whole 16-byte chunks, dZ zero from N to the next chunk.  The
+ * aligned rows of whole 16-byte chunks, dZ zero from N to the next chunk; 256 rows
+ * of dZ in dX, 128 bytes' worth of rows of the other operands, within 2 GiB.  The
  * workspace has void_linear_grad_workspace_bytes(rows and columns of the
  * result, depth of the sum, dtype) bytes. */
 size_t void_linear_grad_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t dtype);

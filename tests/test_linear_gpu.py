@@ -347,6 +347,39 @@ def test_offsets_past_31_bits(gpu):
     close(dx[-70:], want[1], bound[1], "dx")
 
 
+@gpu_only
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [1, 8, 40, 100, 300])
+def test_rows_far_apart(gpu, dtype, M):
+    # The last token of each of M sequences: 256 rows (or all) span more than 2 GiB, where
+    # 31-bit offsets end.  So do a weight's and a gradient's rows.  NaN lies between.
+    N, K = 48, 72
+
+    def far(t):
+        rows, cols = t.shape
+        pitch = (1 << 31) // t.element_size() // min(max(rows, 2), 256) // 64 * 64 + 64
+        buf = torch.full((rows, pitch), float("nan"), dtype=dtype, device=gpu)
+        buf[:, pitch - cols:] = t
+        return buf[:, pitch - cols:]
+
+    x, w, b, r, dy = inputs(gpu, M, N, K, dtype, M)
+    check(far(x), w, b, far(r), dy, "gelu")
+    check(x, w, b, None, far(dy), "none")
+    check(x, far(w), b, r, far(dy), "silu")
+
+
+@gpu_only
+def test_one_row_of_any_pitch(gpu):
+    # x and the gradient of one row: their pitch is never used.
+    x, w, b, r, dy = inputs(gpu, 1, 40, 64, torch.bfloat16)
+    place = lambda t: t.as_strided(t.shape, (1 << 33, 1))
+    check(place(x), w, b, place(r), place(dy), "none")
+    check(place(x), w, b, None, place(dy), "silu")
+    # A weight of one row.
+    x, w, b, r, dy = inputs(gpu, 100, 1, 64, torch.bfloat16)
+    check(x, place(w), b, r, dy, "gelu")
+
+
 def test_refusals():
     x, w = torch.randn(2, 8), torch.randn(4, 8)
     f = void_amd.fused_linear
@@ -384,3 +417,18 @@ def test_abi_refusals():
     assert lib.void_linear_grad_w(at, 40, at, 60, 100, 40, 64, 1, at, 64, None, 0, None) == -2
     assert lib.void_linear_grad_z(at, 40, None, 100, 40, 1, at, 40, None, 1, None, 0, None) == -1
     assert lib.void_linear_grad_z(at, 40, None, 100, 40, 1, None, 0, at, 1, None, 0, None) == -4
+
+
+def test_abi_refuses_rows_out_of_reach():
+    import ctypes
+    from void_amd import _lib
+    lib = _lib.lib()
+    at = 1 << 20  # never read
+    base = dict(x=at, ldx=64, w=at, ldw=64, y=at, ldy=40, M=100, N=40, K=64, dtype=1, bias_dtype=1)
+    for bad in (dict(ldx=1 << 24), dict(ldw=1 << 25)):
+        a = _lib.LinearArgs(**{**base, **bad})
+        assert lib.void_linear(ctypes.byref(a), None) == -2, bad
+    assert lib.void_linear_grad_x(at, 1 << 24, at, 64, 100, 40, 64, 1, at, 64, None, 0, None) == -2
+    assert lib.void_linear_grad_x(at, 40, at, 1 << 26, 100, 40, 64, 1, at, 64, None, 0, None) == -2
+    assert lib.void_linear_grad_w(at, 1 << 25, at, 64, 100, 40, 64, 1, at, 64, None, 0, None) == -2
+    assert lib.void_linear_grad_w(at, 40, at, 1 << 26, 100, 40, 64, 1, at, 64, None, 0, None) == -2

@@ -213,25 +213,28 @@ struct Operand {
   int voff[kLoads];
   int at;               // r of load 0's chunk within a step; turned: kRows more for each next
 
-  // I - i0 rows (turned: columns) remain from i0 on.  Offsets within a step fit 31 bits
-  // (checked by the host).
+  // I - i0 rows (turned: columns) remain from i0 on.  Offsets to the rows that there are fit
+  // 31 bits (checked by the host); those past them may wrap and are not used.
   __device__ __forceinline__ void init(const void* p, int64_t ld, int64_t i0, int64_t I, int64_t r0, int wave,
                                        int lane) {
-    const int id = wave * 64 + lane, pitch = (int)ld * (int)sizeof(E);
+    const int id = wave * 64 + lane;
+    const uint32_t pitch = (uint32_t)ld * (uint32_t)sizeof(E);
     const int rows = (int)std::min<int64_t>(I - i0, B);
     if constexpr (!TURNED) {
       base = static_cast<const uint8_t*>(p) + (i0 * ld + r0) * (int64_t)sizeof(E);
       step = 128;
-      const int row = id >> 3, c = (id & 7) ^ (row & 7), first = row * pitch + 16 * c;
+      const int row = id >> 3, c = (id & 7) ^ (row & 7);
+      const uint32_t first = row * pitch + 16 * c;
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) voff[q] = row + q * kRows < rows ? first + q * kRows * pitch : kOutOfRange;
+      for (int q = 0; q < kLoads; ++q) voff[q] = row + q * kRows < rows ? (int)(first + q * kRows * pitch) : kOutOfRange;
       at = c * kPer;
     } else {
       base = static_cast<const uint8_t*>(p) + (r0 * ld + i0) * (int64_t)sizeof(E);
       step = ld * 128;
-      const int row = id / kCpr, c = (id % kCpr) ^ swizzle(row), first = row * pitch + 16 * c;
+      const int row = id / kCpr, c = (id % kCpr) ^ swizzle(row);
+      const uint32_t first = row * pitch + 16 * c;
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) voff[q] = c * kPer < rows ? first + q * kRows * pitch : kOutOfRange;
+      for (int q = 0; q < kLoads; ++q) voff[q] = c * kPer < rows ? (int)(first + q * kRows * pitch) : kOutOfRange;
       at = row;
     }
   }
@@ -869,6 +872,9 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
 
 template <class E, bool TA, bool TB>
 void product(Product p, const Plan& plan, hipStream_t stream) {
+  // The rows that lda and ldb lie between: of a single one the pitch may be anything.
+  if ((TA ? p.K : p.M) <= 1) p.lda = 0;
+  if ((TB ? p.K : p.N) <= 1) p.ldb = 0;
   p.splits = plan.splits;
   p.steps_per_split = plan.steps_per_split;
   p.tiles_m = (int)((p.M + plan.tile - 1) / plan.tile);
@@ -930,6 +936,12 @@ int check(const void_linear_args* d) {
   return 1;
 }
 
+// Whether 31-bit offsets reach the rows that a step of a tile takes: 256 at most of a
+// plain operand, a step's depth of a turned one.  A single row's pitch is not looked at.
+bool within_reach(int64_t rows, int64_t ld, int esz, bool turned = false) {
+  return rows <= 1 || std::min<int64_t>(rows, turned ? 128 / esz : 256) * ld * esz <= INT_MAX - 65536;
+}
+
 int64_t padded(int64_t cols, int esz) { return (cols * esz + 15) / 16 * 16 / esz; }
 
 }  // namespace
@@ -963,14 +975,14 @@ int void_linear(const void_linear_args* d, hipStream_t stream) {
     return void_internal_fail(VOID_ERR_ARG, "arrays must be aligned to their elements");
   const Epilogue epi{d->y, d->ldy, d->bias, d->residual, d->ldr, d->slope, d->bias_dtype == VOID_DT_F32, d->activation};
   const bool whole = d->K == 0 || (whole_chunks(d->x, d->ldx, d->K, esz) && whole_chunks(d->w, d->ldw, d->K, esz));
-  if (few_by_rows(d->M, d->N, d->K, esz, whole)) {
+  const bool near = d->K == 0 || (within_reach(d->M, d->ldx, esz) && within_reach(d->N, d->ldw, esz));
+  if (few_by_rows(d->M, d->N, d->K, esz, whole && near)) {
     by_type(d->dtype, [&](auto e) { few<decltype(e)>(d, epi, stream); });
     return launched();
   }
   if (!whole)
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "more than 64 tokens need rows of whole 16-byte chunks");
-  if (256 * std::max(d->ldx, d->ldw) * esz > INT_MAX - 65536)
-    return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
+  if (!near) return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
   const Plan plan = plan_of(d->M, d->N, d->K, esz);
   if (plan.splits > 1 && (!d->workspace || (uintptr_t)d->workspace % 4 ||
                           d->workspace_bytes < (size_t)plan.splits * d->M * d->N * 4))
@@ -998,7 +1010,7 @@ int void_linear_grad_x(const void* dz, int64_t ldz, const void* w, int64_t ldw, 
   if (N && (!whole_chunks(dz, ldz, padded(N, esz), esz) || ldz < padded(N, esz) ||
             !whole_chunks(w, ldw, padded(K, esz), esz) || ldw < padded(K, esz)))
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "the products of the gradient need rows of whole 16-byte chunks");
-  if (256 * std::max(ldz, ldw) * esz > INT_MAX - 65536)
+  if (N && !(within_reach(M, ldz, esz) && within_reach(N, ldw, esz, true)))
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
   const Plan plan = plan_of(M, K, N, esz);
   if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)plan.splits * M * K * 4))
@@ -1027,7 +1039,7 @@ int void_linear_grad_w(const void* dz, int64_t ldz, const void* x, int64_t ldx, 
   if (M && (!whole_chunks(dz, ldz, padded(N, esz), esz) || ldz < padded(N, esz) ||
             !whole_chunks(x, ldx, padded(K, esz), esz) || ldx < padded(K, esz)))
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "the products of the gradient need rows of whole 16-byte chunks");
-  if (256 * std::max(ldz, ldx) * esz > INT_MAX - 65536)
+  if (M && !(within_reach(M, ldz, esz, true) && within_reach(M, ldx, esz, true)))
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
   const Plan plan = plan_of(N, K, M, esz);
   if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)plan.splits * N * K * 4))

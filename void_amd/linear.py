@@ -39,12 +39,29 @@ def _whole(cols: int, t: torch.Tensor) -> int:
     return -(-cols // per) * per
 
 
+_REACH = (1 << 31) - 1 - (1 << 16)  # bytes that 256 rows of the tiles' operands may span
+
+
+def _far(t: torch.Tensor) -> bool:
+    """Whether the rows of t (2-D) lie further apart than the tiles' 31-bit offsets reach."""
+    R = t.shape[0]
+    return R > 1 and min(R, 256) * t.stride(0) * t.element_size() > _REACH
+
+
+def _padded(t: torch.Tensor, zero_tail: bool = False) -> torch.Tensor:
+    """_runtime.padded_rows, copied too where the rows lie too far apart and a copy's do not."""
+    rows = _runtime.padded_rows(t, zero_tail=zero_tail)
+    if rows is t and t.numel() and _far(t) and t.stride(0) > _whole(t.shape[1], t):
+        return _runtime.padded_copy(t, _whole(t.shape[1], t))
+    return rows
+
+
 def _chunked(t: torch.Tensor) -> torch.Tensor:
     """t with rows that can be read to the end of their last 16-byte chunk, whatever lies there."""
-    rows = _runtime.padded_rows(t)
+    rows = _padded(t)
     end = rows.storage_offset() + (rows.shape[0] - 1) * rows.stride(0) + _whole(rows.shape[1], rows)
     if rows is t and end * t.element_size() > t.untyped_storage().nbytes():
-        return _runtime.padded_rows(t, zero_tail=True)  # the storage ends inside the last row's last chunk
+        return _padded(t, zero_tail=True)  # the storage ends inside the last row's last chunk
     return rows
 
 
@@ -56,12 +73,13 @@ def _forward(x, weight, bias, residual, code: int, with_slope: bool):
     M = rows.shape[0]
     if lib.void_linear_any_alignment(M):
         rows = _runtime.flat_rows(rows)
-        if M > 1 and rows.stride(0) < K:
+        # Few rows far apart are copied for the tiles; a weight's stay, which few_kernel reads.
+        if M > 1 and (rows.stride(0) < K or _far(rows)):
             rows = rows.contiguous()
         w = weight if weight.stride(1) == 1 and weight.stride(0) >= K else weight.contiguous()
         depth = K
     else:
-        rows, w = _runtime.padded_rows(rows, zero_tail=True), _runtime.padded_rows(weight, zero_tail=True)
+        rows, w = _padded(rows, zero_tail=True), _padded(weight, zero_tail=True)
         depth = _whole(K, x)
     y = x.new_empty(x.shape[:-1] + (N,))
     slope = None
@@ -121,7 +139,7 @@ class _FusedLinear(Function):
         dz = None
         if need_x or need_w:
             if slope is None:
-                dz = dy = _runtime.padded_rows(dy, zero_tail=True)
+                dz = dy = _padded(dy, zero_tail=True)
             else:
                 dz = torch.empty(M, _whole(N, grad), dtype=dtype, device=dev)
         if slope is not None or need_b:
@@ -160,7 +178,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     (another type than x's is widened to fp32); residual has the result's shape
     [..., N] and x's type.  activation: "none", "relu", "gelu" (tanh form) or
     "silu".  Any strides are taken; for more than 64 rows, operands whose rows
-    are not whole 16-byte chunks are copied to such once.  Gradients flow to all
+    are not whole 16-byte chunks are copied to such once, and so are rows so far
+    apart that 256 of them (or all) span 2 GiB.  Gradients flow to all
     four tensors and are not differentiable themselves.
     """
     code = _code(activation)
