@@ -475,7 +475,8 @@ typedef struct void_linear_args {
   void* y;
   int64_t ldy;
   void* slope;            /* [M, N] contiguous activation'(Z) for the gradient: fp32 for fp32
-                             values, else 2-byte codes; needs an activation */
+                             values, else 2-byte codes (within 2^-16, and within 2^-10 of
+                             themselves from 2^-29 on); needs an activation */
   void* workspace;
   size_t workspace_bytes; /* void_linear_workspace_bytes(); no initial contents */
   int64_t M, N, K;

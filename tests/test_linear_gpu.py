@@ -229,6 +229,44 @@ def test_non_finite_values_stay_alone(gpu, M, name):
 
 
 @gpu_only
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [7, 130])
+@pytest.mark.parametrize("name,low,high", [("silu", -16.0, -7.0), ("gelu", -4.8, -3.2)])
+def test_saturated_units_keep_their_gradients(gpu, dtype, M, name, low, high):
+    # Units whose slope is 2^-24 to 0.03: relative bounds.  The slope is kept to 2^-10 of
+    # itself from 2^-29 on; an error of z changes it by at most 8 of that relative (2 u' + 1 <=
+    # 8 for gelu, 1 for silu); its own arithmetic rounds an exponent below 32 in 2^-24 steps a
+    # few times, 2^-17 in all; dZ rounds once more before the products.
+    N, K = 48, 64
+    x, w, _, _, dy = inputs(gpu, M, N, K, dtype, 5)
+    w = w * 0.125
+    b = torch.linspace(low, high, N, device=gpu).to(dtype)
+    dy = dy.sign() * (dy.abs() + 0.25) * 8192  # as a loss scaler: dZ stays a normal fp16 value
+    a = [t.detach().requires_grad_() for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(void_amd.fused_linear(*a, name), a, dy)
+    X, W, D = x.double(), w.double(), dy.double()
+    z = X @ W.t() + b.double()
+    ez = (K + 32) * EPS32 * (X.abs() @ W.abs().t()) + 2 * EPS32 * (z.abs() + b.double().abs())
+    if name == "silu":
+        s = torch.sigmoid(z)
+        slope = s * (1 + z * torch.sigmoid(-z))
+    else:
+        v = 1.5957691216 * (z + 0.044715 * z ** 3)
+        s = torch.sigmoid(v)
+        slope = s * (1 + z * torch.sigmoid(-v) * 1.5957691216 * (1 + 0.134145 * z * z))
+    assert (slope < 0).all() and slope.abs().min() > 2.0 ** -24 and slope.abs().max() < 0.03
+    dz = D * slope
+    es = (2.0 ** -10 + 8 * ez + 2.0 ** -17) * dz.abs()
+    edz = es + U[dtype] * dz.abs()
+    close(db, dz.sum(0), (es + (M + 32) * EPS32 * dz.abs()).sum(0) + U[dtype] * dz.sum(0).abs(), "db")
+    for got, left, right, what in ((dw, dz.t(), X, "dw"), (dx, dz, W, "dx")):
+        el = edz.t() if what == "dw" else edz
+        want = left @ right
+        bound = el @ right.abs() + (max(M, N) + 32) * EPS32 * (left.abs() @ right.abs()) + U[dtype] * want.abs()
+        close(got, want, bound, what)
+
+
+@gpu_only
 @pytest.mark.parametrize("M", [7, 130])
 @pytest.mark.parametrize("name", ["none", "gelu", "silu"])
 def test_gradients_against_differences(gpu, M, name):

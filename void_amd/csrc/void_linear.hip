@@ -35,18 +35,32 @@ typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 
 // ---- epilogue --------------------------------------------------------------
 
-// act'(Z), kept for the backward pass: fp32 for fp32 values, else 16-bit fixed
-// point 2^15 s + 2^13 (s lies in [-0.13, 1.13] for every activation; 0 and 1 are
-// exact, others within 2^-16: a tenth of a bf16 rounding of dZ, where a slope
-// rounded to bf16 would add another whole one).  NaN becomes 0, which no slope takes.
+// act'(Z), kept for the backward pass: fp32 for fp32 values, else a 16-bit code.  s lies
+// in [-0.13, 1.13] for every activation.  From 2^-5 on |s| is fixed point in steps of 2^-15
+// (within 2^-16; 1 is exact), which takes 37000 codes of the positive side and 3200 of the
+// negative; the others hold |s| from 2^-29 to 2^-5 with 9 bits behind its leading one
+// (within 2^-10 of itself), so that saturated units, whose slopes are small, keep their
+// gradients; below that it is 0.  Beside dZ's rounding (2^-8 of itself for bf16, 2^-11 for
+// fp16) that is a quarter at most for bf16, and for fp16 a thirtieth near 1, as much at 2^-5
+// and twice as much below.  NaN becomes 0, which no slope takes.  Packing costs 1.3 % of a
+// training step of 8192 x 14336 x 4096 with GELU against fixed point alone, which rounds
+// slopes below 2^-16 to 0 (2605 us and 2570).
 template <class E>
 struct Slope {
   typedef uint16_t type;
+  static constexpr uint32_t kLow = 0x31000000;  // 2^-29
   static __device__ __forceinline__ uint16_t pack(float s) {
-    return (uint16_t)__float2uint_rz(fmaf(s, 32768.f, 8192.5f));
+    const float a = fabsf(s);
+    const uint32_t code = (max(__float_as_uint(a), kLow) - kLow + (1 << 13)) >> 14;  // 0 .. 12288 below 2^-5
+    const float m = a < 0x1p-5f ? (float)code : fmaf(a, 32768.f, 11264.f);
+    return (uint16_t)__float2uint_rz(16384.5f + copysignf(m, s));
   }
   static __device__ __forceinline__ float unpack(uint16_t u) {
-    return u ? fmaf((float)u, 1.f / 32768.f, -0.25f) : __builtin_nanf("");
+    const int w = (int)u - 16384;
+    const uint32_t m = (uint32_t)abs(w);
+    const float small = m ? __uint_as_float((m << 14) + kLow) : 0.f;
+    const float a = m < 12288 ? small : (float)((int)m - 11264) * 0x1p-15f;
+    return u ? (w < 0 ? -a : a) : __builtin_nanf("");
   }
 };
 template <>

@@ -8,7 +8,8 @@ only (void/fusion.py:98-304), without the residual and without gradients.
 
 Products are summed in fp32 and Y is rounded once.  The forward pass keeps
 activation'(Z) for the backward pass (fp32, or 2 bytes a value for 16-bit
-inputs); dZ is rounded to the inputs' type, which the matrix cores take.
+inputs: within 2^-16, and from 2^-29 on within 2^-10 of itself); dZ is rounded
+to the inputs' type, which the matrix cores take.
 """
 
 from __future__ import annotations
