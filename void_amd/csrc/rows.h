@@ -155,6 +155,14 @@ __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, Q...>) {
   (f(std::integral_constant<int, Q>{}), ...);
 }
 
+// Between LDS writes of some lanes of a wave and reads of them by others: the wave's LDS
+// operations run in order, this keeps the compiler to it.  Costs no instruction.
+__device__ __forceinline__ void lanes_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Sum over the aligned group of T lanes (a power of two up to 64) that holds this lane.
 template <int T>
 __device__ __forceinline__ float lanes_sum(float v) {

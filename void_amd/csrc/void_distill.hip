@@ -175,6 +175,7 @@ __device__ __forceinline__ float teacher_by_wave(const Args& a, const Entries& e
     if (p != 0.f) own += p * (d / a.temperature - log_sum);  // log p
     en.t[j] = p;
   }
+  lanes_in_order();  // equal indices' p are other lanes'
   for (int j = lane; j < a.k; j += 64) {
     const int at = en.at[j];
     if (at < lo || at >= hi) continue;
@@ -303,8 +304,9 @@ __device__ __forceinline__ void zero_slice(E* ds, const Slice<E>& sl) {
   if (threadIdx.x < sl.rest) ds[(int64_t)sl.last * Piece<E>::n + threadIdx.x] = (E)0.f;
 }
 
-// A row's entries into LDS, with its logits there where it has any; its flags.  Ends
-// behind a barrier that the entries are behind too (the logits only where `wait`).
+// A row's entries into LDS, with its logits there where it has any; its flags.  Every
+// thread's entries stand before the barrier here, the logits (en.s) behind it: where other
+// lanes read those, another barrier comes first.
 template <class E, int T>
 __device__ __forceinline__ int take_entries(const Args& a, int64_t row, const E* s, const Entries& en, Areas& red) {
   __syncthreads();  // en is free

@@ -333,6 +333,7 @@ struct Place {
 template <class E, int COLS, int ROWS, int PITCH = COLS>
 __device__ __forceinline__ void store_strip(const Product& p, int split, const float* strip, int64_t row0, int64_t col0,
                                             int lane) {
+  lanes_in_order();  // the strip is other lanes' writing
   constexpr int n = Piece<E>::n, kLanes = COLS / n, kRows = 64 / kLanes, kAhead = ROWS / kRows < 4 ? ROWS / kRows : 4;
   static_assert(ROWS % (kAhead * kRows) == 0);
   typedef typename Piece<E>::fvec F;
@@ -548,6 +549,7 @@ __global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
   each_of(
       [&](auto h_) {
         constexpr int h = 2 * decltype(h_)::value;
+        lanes_in_order();  // the strip is read
 #pragma unroll
         for (int j = 0; j < R; ++j) {
           to_strip<128>(strip, 32 * j, acc[h][j], lane);
@@ -639,6 +641,7 @@ __global__ __launch_bounds__(256, 1) void wide_plain_kernel(Product p) {
   each_of(
       [&](auto h_) {
         constexpr int h = 4 * decltype(h_)::value;
+        lanes_in_order();  // the strip is read
         // Lane (j, g) holds column j and rows 4 g .. 4 g + 3 of each 16 x 16.
 #pragma unroll
         for (int i = 0; i < 4; ++i)
