@@ -418,6 +418,33 @@ def test_one_row_of_any_pitch(gpu):
     check(x, place(w), b, r, dy, "gelu")
 
 
+@gpu_only
+def test_more_columns_than_one_grid_axis_holds(gpu):
+    # 2^24 groups of 16 rows of W, and of 64 columns' sums: more than 2^32 threads along one axis.
+    N, K = (1 << 28) + 37, 2
+    w = torch.randn(N, K, device=gpu, dtype=torch.bfloat16)
+    b = torch.randn(N, device=gpu, dtype=torch.bfloat16).requires_grad_()
+    x, dy = torch.randn(1, K, device=gpu).to(w.dtype), torch.randn(1, N, device=gpu, dtype=w.dtype)
+    y = void_amd.fused_linear(x, w, b, "gelu")
+    db, = torch.autograd.grad(y, b, dy)
+    for part in (slice(0, 70), slice((1 << 27) - 40, (1 << 27) + 40), slice(N - 70, N)):
+        want, bound = reference(x, w[part], b.detach()[part], None, dy[:, part], "gelu")
+        close(y.detach()[:, part], want[0], bound[0], "y")
+        close(db[part], want[3], bound[3] + U[b.dtype] * want[3].abs(), "db")
+
+
+@gpu_only
+def test_more_tiles_than_one_grid_axis_holds(gpu):
+    # 2^24 tiles of 64 rows: more than 2^32 threads along one axis.
+    M, N, K = (1 << 30) + 40, 3, 8
+    g, w, b, _, _ = inputs(gpu, 1000, N, K, torch.bfloat16)
+    x = g.repeat(-(-M // 1000), 1)[:M]
+    y = void_amd.fused_linear(x, w, b, "silu")
+    for part in (slice(0, 90), slice((1 << 29) - 40, (1 << 29) + 40), slice(M - 90, M)):
+        want, bound = reference(x[part], w, b, None, None, "silu")
+        close(y[part], want[0], bound[0], "y")
+
+
 def test_refusals():
     x, w = torch.randn(2, 8), torch.randn(4, 8)
     f = void_amd.fused_linear

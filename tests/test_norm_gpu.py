@@ -281,6 +281,25 @@ def test_offsets_past_31_bits(gpu):
     close(ends[2], rx, ex, "dx")
 
 
+@gpu_only
+def test_rows_of_more_columns_than_one_grid_axis_sums(gpu):
+    # 2^26 groups of 64 columns' sums are more than 2^32 threads along one axis of a grid.
+    C = (1 << 27) + 37
+    x = torch.randn(C, device=gpu, dtype=torch.bfloat16)[None]
+    dy = torch.randn(C, device=gpu, dtype=torch.bfloat16)[None]
+    w, b = (torch.randn(C, device=gpu, dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    dw, db = torch.autograd.grad(void_amd.layer_norm(x, w, b), (w, b), dy)
+    # One row: its own terms, at both ends and at the places that would be another's.
+    mean, var = x.double().mean(), x.double().var(correction=0)
+    for part in (slice(0, 70), slice((1 << 26) - 40, (1 << 26) + 40), slice(C - 70, C)):
+        h = (x[0, part].double() - mean) / torch.sqrt(var + 1e-5)
+        want = dy[0, part].double() * h
+        # Sums of 2^27 values in 1024 threads: 2^14 terms each; the row's mean is near 0.
+        bound = (1 << 15) * EPS32 * dy[0, part].double().abs() * (h.abs() + 1) + U[torch.bfloat16] * want.abs()
+        close(dw[part], want, bound, "dw")
+        assert torch.equal(db[part], dy[0, part])
+
+
 def test_refusals():
     x = torch.randn(2, 8)
     with pytest.raises(RuntimeError, match="GPU"):

@@ -210,6 +210,15 @@ struct RowSum {
   }
 };
 
+// Grids of any number of workgroups: along one axis their threads have to stay below 2^32
+// (a launch of more runs what is left of that, without an error), so that from 2^20
+// workgroups on they go on along the second.
+constexpr int64_t kGridX = 1 << 20;
+inline dim3 grid_of(int64_t blocks) {
+  return dim3((unsigned)(blocks < kGridX ? blocks : kGridX), (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ int64_t grid_block() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
+
 // Column c of n rows of `pitch` floats, added in order by a workgroup of 1024: each
 // wave every 16th row, eight of them in flight, then the waves in order.  The result
 // is the first wave's (0 past the last column).

@@ -694,7 +694,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(const E* __restrict__ x, i
   __shared__ v4f sum[NW][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = grid_block() * 16;  // the last groups of a grid of two axes may lie past N
   // Rows past the end repeat the last one; their sums are not stored.
   const E* wr = w + std::min<int64_t>(n0 + i, N - 1) * ldw + g * kPer;
   const E* xr[MT];
@@ -812,7 +812,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const E* __restrict__ dy, in
 template <class W>
 __global__ __launch_bounds__(1024) void bias_sum_kernel(const float* __restrict__ part, int n, int N, W* __restrict__ db) {
   __shared__ float sum[16][64];
-  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int64_t c = grid_block() * 64 + (threadIdx.x & 63);
   const float s = partial_rows_sum(part, n, N, c, sum);
   if (threadIdx.x < 64 && c < N) db[c] = (W)s;
 }
@@ -841,10 +841,11 @@ struct Plan {
   int tile, splits, steps_per_split;
 };
 
-// The plan of least estimated time, in microseconds.  A CU takes one 256-row tile at
-// a time, or two of the others: `fixed` is a tile's start and epilogue, `alone` and
-// `full` a step of 128 bytes along r where a CU has one tile and, per tile, where it
-// has two; splits add a launch and their sums' traffic.  The figures are fitted to 400
+// The plan of least estimated time, in microseconds, of those with at most kMaxTiles
+// workgroups (of 256 threads: below 2^32 along a grid's axis); tile 0 where there is none.
+// A CU takes one 256-row tile at a time, or two of the others: `fixed` is a tile's start
+// and epilogue, `alone` and `full` a step of 128 bytes along r where a CU has one tile and,
+// per tile, where it has two; splits add a launch and their sums' traffic.  The figures are fitted to 400
 // timings of 18 bf16 and 8 fp32 products (17 to 8192 rows, 512 to 14336 columns, depths
 // of 512 to 14336; the estimates are within 15 %, but for products of several rounds of
 // 256-row tiles, which the chip's power makes up to a fifth slower; the plans chosen are
@@ -860,6 +861,8 @@ constexpr Cost kCost16[] = {{256, 11.7, 1.17, 1.17, 3.0, 1.2},
                             {32, 1.9, 0.35, 0.29, 5.0, 0.85}};
 constexpr Cost kCost32[] = {{128, 1.3, 2.07, 1.96, 4.8, 1.0}, {64, 1.0, 1.12, 1.03, 4.5, 1.15}, {32, 2.7, 0.65, 0.57, 3.0, 1.0}};
 
+constexpr int64_t kMaxTiles = (1 << 24) - 1;
+
 Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
   const int64_t steps = std::max<int64_t>(1, (K * esz + 127) / 128);
   Plan best{};
@@ -869,7 +872,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int esz) {
     const int64_t tiles = ((M + c.tile - 1) / c.tile) * ((N + width - 1) / width);
     for (int splits = 1; splits <= 32 && splits <= steps; ++splits) {
       const int64_t per = (steps + splits - 1) / splits;
-      if (splits > 1 && ((steps + per - 1) / per != splits || per < 4)) continue;
+      if (tiles * splits > kMaxTiles || (splits > 1 && ((steps + per - 1) / per != splits || per < 4))) continue;
       const int64_t each = (tiles * splits + kCus - 1) / kCus;  // tiles of the fullest CU
       const double one = c.fixed + per * c.alone, two = c.fixed + per * std::max(c.alone, 2 * c.full);
       double cost = c.tile == 256 ? each * one : each / 2 * two + each % 2 * (one - 0.3 * c.fixed);
@@ -915,8 +918,8 @@ void few(const void_linear_args* d, const Epilogue& epi, hipStream_t stream) {
   auto go = [&](auto mt, auto nw) {
     constexpr int MT = decltype(mt)::value, NW = decltype(nw)::value;
     by_parity<E>(d->x, d->ldx, d->w, d->ldw, std::max(d->M, d->N), [&](auto odd) {
-      hipLaunchKernelGGL((few_kernel<E, MT, NW, decltype(odd)::value>), dim3((unsigned)((d->N + 15) / 16)), dim3(64 * NW),
-                         0, stream, static_cast<const E*>(d->x), d->ldx, static_cast<const E*>(d->w), d->ldw, (int)d->M,
+      hipLaunchKernelGGL((few_kernel<E, MT, NW, decltype(odd)::value>), grid_of((d->N + 15) / 16), dim3(64 * NW), 0,
+                         stream, static_cast<const E*>(d->x), d->ldx, static_cast<const E*>(d->w), d->ldw, (int)d->M,
                          d->N, (int)d->K, epi);
     });
   };
@@ -1001,6 +1004,7 @@ int void_linear(const void_linear_args* d, hipStream_t stream) {
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "more than 64 tokens need rows of whole 16-byte chunks");
   if (!near) return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
   const Plan plan = plan_of(d->M, d->N, d->K, esz);
+  if (!plan.tile) return void_internal_fail(VOID_ERR_UNSUPPORTED, "more tiles than a grid holds");
   if (plan.splits > 1 && (!d->workspace || (uintptr_t)d->workspace % 4 ||
                           d->workspace_bytes < (size_t)plan.splits * d->M * d->N * 4))
     return void_internal_fail(VOID_ERR_WORKSPACE, "linear: workspace missing or too small");
@@ -1030,6 +1034,7 @@ int void_linear_grad_x(const void* dz, int64_t ldz, const void* w, int64_t ldw, 
   if (N && !(within_reach(M, ldz, esz) && within_reach(N, ldw, esz, true)))
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
   const Plan plan = plan_of(M, K, N, esz);
+  if (!plan.tile) return void_internal_fail(VOID_ERR_UNSUPPORTED, "more tiles than a grid holds");
   if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)plan.splits * M * K * 4))
     return void_internal_fail(VOID_ERR_WORKSPACE, "linear gradient: workspace missing or too small");
   by_type(dtype, [&](auto e) {
@@ -1059,6 +1064,7 @@ int void_linear_grad_w(const void* dz, int64_t ldz, const void* x, int64_t ldx, 
   if (M && !(within_reach(M, ldz, esz, true) && within_reach(M, ldx, esz, true)))
     return void_internal_fail(VOID_ERR_UNSUPPORTED, "rows are too far apart");
   const Plan plan = plan_of(N, K, M, esz);
+  if (!plan.tile) return void_internal_fail(VOID_ERR_UNSUPPORTED, "more tiles than a grid holds");
   if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < (size_t)plan.splits * N * K * 4))
     return void_internal_fail(VOID_ERR_WORKSPACE, "linear gradient: workspace missing or too small");
   by_type(dtype, [&](auto e) {
@@ -1114,7 +1120,7 @@ int void_linear_grad_z(const void* dy, int64_t lddy, const void* slope, int64_t 
                            db ? static_cast<float*>(workspace) : nullptr);
       });
     if (db) {
-      const dim3 grid((unsigned)((N + 63) / 64));
+      const dim3 grid = grid_of((N + 63) / 64);
       if (bias_dtype == VOID_DT_F32)
         hipLaunchKernelGGL(bias_sum_kernel<float>, grid, dim3(1024), 0, stream, static_cast<float*>(workspace), gy,
                            (int)N, static_cast<float*>(db));

@@ -341,7 +341,7 @@ template <class W>
 __global__ __launch_bounds__(1024) void norm_sum_kernel(const float* __restrict__ part, int n, int cols,
                                                         W* __restrict__ dw, W* __restrict__ db) {
   __shared__ float sum[16][64];
-  const int64_t j = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int64_t j = grid_block() * 64 + (threadIdx.x & 63);
   const float s = partial_rows_sum(part, n, 2 * (int64_t)cols, j, sum);
   if (threadIdx.x < 64) {
     if (j < cols) {
@@ -432,7 +432,7 @@ void backward(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const 
                          stream, dy, lddy, x, ldx, stats, rows, cols, part);
   }
   if (part)
-    hipLaunchKernelGGL(norm_sum_kernel<W>, dim3((unsigned)((2 * (int64_t)cols + 63) / 64)), dim3(1024), 0, stream, part,
+    hipLaunchKernelGGL(norm_sum_kernel<W>, grid_of((2 * (int64_t)cols + 63) / 64), dim3(1024), 0, stream, part,
                        n, cols, static_cast<W*>(dw), static_cast<W*>(db));
 }
 
@@ -516,7 +516,7 @@ int void_layer_norm_grad(const void* dy, int64_t lddy, const void* x, int64_t ld
       backward<E, W>(dy, lddy, x, ldx, weight, stats, rows, cols, dx, lddx, dweight, dbias,
                      params ? static_cast<float*>(workspace) : nullptr, stream);
     else  // no rows: the parameters' gradients are sums of nothing
-      hipLaunchKernelGGL(norm_sum_kernel<W>, dim3((unsigned)((2 * (int64_t)cols + 63) / 64)), dim3(1024), 0, stream,
+      hipLaunchKernelGGL(norm_sum_kernel<W>, grid_of((2 * (int64_t)cols + 63) / 64), dim3(1024), 0, stream,
                          nullptr, 0, cols, static_cast<W*>(dweight), static_cast<W*>(dbias));
   });
   return launched();
