@@ -334,8 +334,9 @@ __device__ __forceinline__ int take_entries(const Args& a, int64_t row, const E*
 // ---- kernels ---------------------------------------------------------------
 
 // Unit u = (row, slice).  Writes the slice's part; used[row] (slice 0).  With
-// LOSS (S = 1) the row's loss too.  Clears `arrived` (unless null).  Bound by reading the logits: 4096 x 32768 bf16
-// 52 us, 5.2 TB/s; 730 x 50021 fp32 with a quarter of the rows without entries 24 us,
+// LOSS (S = 1) the row's loss too.  Clears `arrived` (unless null).  Bound by reading the
+// logits: 4096 x 32768 bf16 63 us between other work, 4.2 TB/s (52 us call after call, partly
+// from the caches); 730 x 50021 fp32 with a quarter of the rows without entries 24.5 us,
 // 4.5 TB/s.
 template <class E, int T, bool LOSS, bool ODD>
 __global__ __launch_bounds__(T) void distill_parts_kernel(Args a, int S, int64_t units, float2* __restrict__ parts,
@@ -431,7 +432,7 @@ __device__ __forceinline__ void add_row_loss(const Args& a, int64_t row, float l
 // null) divides by the number of rows with entries.  With `loss`, slice 0
 // writes the row's loss; `total` (unless null) becomes their sum or mean.  Bound by
 // one read of the logits and one write of as much: 4096 x 32768 bf16 102 us, 5.3 TB/s;
-// 730 x 50021 fp32 with a quarter of the rows without entries 58 us, 4.4 TB/s.  What
+// 730 x 50021 fp32 with a quarter of the rows without entries 55 us, 4.7 TB/s.  What
 // the entries need of the teacher is made while the logits come (300 x 131072 bf16,
 // loss and gradient: 50.4 us, and 54.4 at the end).
 template <class E, int T, bool ODD>
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(1024) void distill_count_kernel(Args a, int32_t* __
 // read again from the caches.  Four waves a SIMD: while one workgroup sums, others
 // load and store.  Bound by the memory: 8192 x 65536 bf16 466 us, 4.6 TB/s of one read
 // and one write; x 131072 967 us, 4.45, with a quarter of the rows without entries
-// 820 to 870 us, 4.3 to 4.6 (a copy of 2 GiB: 4.94).
+// 820 to 870 us, 4.3 to 4.6 (a copy of 2 GiB: 4.94); 2048 x 65536 fp32 239 us, 4.5.
 template <class E, int T, int NV, bool ODD>
 __global__ __launch_bounds__(T, 4) void distill_step_kernel(Args a, float scale, const int32_t* __restrict__ counts,
                                                             int n_counts, E* __restrict__ grad, int64_t ldg,

@@ -382,7 +382,8 @@ __device__ __forceinline__ void to_strip(float* strip, int col, v16f acc, int la
 // since there the operand that streams past is what bounds it, and bytes in flight
 // what that asks for.  fp32 runs at 137 TFLOP/s in its loop (the instructions' peak is
 // 157): 730 x 5003 x 3001 199 us, 110 TFLOP/s with the tiles' ends.  32 tokens x 14336 x
-// 4096 bf16 29 us, 4.0 TB/s of W.
+// 4096 bf16 29 us, 4.0 TB/s of W; 16 tokens of the same fp32 44 us, 5.4 TB/s.  4096 x 4096 bf16:
+// 128 tokens 21 us, 512 30, 1024 53 in whole calls, of which a join takes 4 to 8.
 template <class E, int BM, bool TA, bool TB>
 __global__ __launch_bounds__(256, 2) void product_kernel(Product p) {
   constexpr int BN = 128, NW = 4, kBK = 128 / (int)sizeof(E), kStages = BM == 128 ? 2 : BM == 64 ? 3 : 4;
@@ -468,9 +469,10 @@ __device__ __forceinline__ void each8(F f) {
 // before its last set, when all of the step has been read and the next step has
 // landed.  LDS holds three steps of A and two of B (all 160 KB): the loads of a step
 // are spread over the sets, four each, so that no wave waits to issue them, and the
-// waits count those of A for the step after next, which stay in flight.  Bound by the
-// chip's power (the clock falls to 1.6 GHz under it): 8192 x 4096 x 14336 bf16 (dX) 717
-// to 790 us, 1220 to 1340 TFLOP/s; 14336 x 4096 x 8192 (dW, both turned) 780 to 810 us.
+// waits count those of A for the step after next, which stay in flight.  8192 x 4096 x 14336
+// bf16 (dX) 717 to 790 us, 1220 to 1340 TFLOP/s; 14336 x 4096 x 8192 (dW, both turned) 780 to
+// 810 us.  The matrix cores are busy 70 % (dX) and 59 % (dW) of the cycles, at 1.8 to 2.0 GHz
+// with random operands: power takes the rest of the 2.4 GHz at which equal values run.
 template <class E, bool TA, bool TB>
 __global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
   constexpr int B = 256, NW = 4, kBK = 64, R = 4, kOperand = B * 128;
@@ -561,9 +563,9 @@ __global__ __launch_bounds__(256, 1) void wide_product_kernel(Product p) {
 }
 
 // The same for two plain operands on the 16 x 16 x 32 instructions, whose sums cost
-// the matrix cores less energy (they take half as many steps along r); the chip runs
-// these tiles at its power limit: 8192 x 14336 x 4096 bf16 725 us, 1327 TFLOP/s, against
-// 773.  (Turned operands' fragments leave too few registers for it.)  A step is two
+// the matrix cores less energy (they take half as many steps along r): 8192 x 14336 x 4096
+// bf16 725 us, 1327 TFLOP/s, against 773; the matrix cores are busy 66 % of the cycles at
+// 2.0 GHz, which power sets.  (Turned operands' fragments leave too few registers for it.)  A step is two
 // fragment sets and takes 1.37 us; a tile's start and end take 12 to 16 us, with GELU and
 // its slope 10 more, which one wave a SIMD spends on them alone.
 template <class E>
@@ -684,7 +686,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // Up to 16 MT tokens: bound by reading W once.  A workgroup of NW waves takes 16
 // rows of W, each wave a share of K straight from memory into fragments (no LDS:
 // nothing of W is used twice), any alignment; the waves' sums are added in order.
-// One token x 14336 x 4096 bf16 25.6 us, 4.6 TB/s.
+// One token x 14336 x 4096 bf16 25.6 us, 4.6 TB/s; fp32 43.8 us, 5.4 TB/s; 16 tokens x 4096 x
+// 4096 fp32 18.5 us, 3.6 TB/s.
 template <class E, int MT, int NW, bool ODD>
 __global__ __launch_bounds__(64 * NW) void few_kernel(const E* __restrict__ x, int64_t ldx, const E* __restrict__ w,
                                                       int64_t ldw, int M, int64_t N, int K, Epilogue epi) {
